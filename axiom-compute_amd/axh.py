@@ -119,6 +119,17 @@ class _BenchOp(ctypes.Structure):
     ]
 
 
+class _RouteOptions(ctypes.Structure):
+    _fields_ = [("n_experts", ctypes.c_uint32), ("top_k", ctypes.c_uint32),
+                ("score", ctypes.c_uint32), ("n_groups", ctypes.c_uint32),
+                ("groups_kept", ctypes.c_uint32), ("group_best", ctypes.c_uint32),
+                ("normalize", ctypes.c_uint32), ("scale", ctypes.c_float)]
+
+
+# Element types of the MXFP4 and expert operations (ggml type ids).
+GGML_F32, GGML_F16, GGML_BF16, GGML_MXFP4 = 0, 1, 30, 39
+SCORES = {"softmax": 0, "sigmoid": 1}
+
 BENCH_OPS = {"q4k": 1, "q4_0": 2, "q5k": 3, "q6k": 4, "gate_up": 5, "matmul_f16": 6,
              "matmul_f32": 7, "read_floor": 8, "launch_empty": 9, "read_shape": 10,
              "gate_up_q4_0": 11, "gate_up_q5k": 12}
@@ -246,6 +257,23 @@ def load_library(path: Optional[Path] = None) -> ctypes.CDLL:
         "axh_q4_0_matvec_variant_count": (u32, []),
         "axh_q4_0_matvec_variant_at": (st, [u32, c.POINTER(_Variant)]),
         "axh_builtin_code_object": (vp, [c.POINTER(sz)]),
+        "axh_mxfp4_quantize": (st, [vp, u32, vp, u64, vp, vp, u32, u32, vp]),
+        "axh_mxfp4_dequant": (st, [vp, vp, vp, u32, vp, u64, vp]),
+        "axh_mxfp4_unpack_ggml": (st, [vp, vp, vp, vp, u64, vp]),
+        "axh_mxfp4_matvec": (st, [vp, vp, vp, vp, vp, u32, u32, vp]),
+        "axh_mxfp4_matmul": (st, [vp, vp, vp, vp, vp, u32, vp, u32, u32, u32, vp]),
+        "axh_mxfp4_matmul_kernel_name": (st, [u32, u32, u32, u32, c.c_char_p, sz]),
+        "axh_expert_route": (st, [vp, u32, vp, vp, vp, vp, u32, c.POINTER(_RouteOptions), vp]),
+        "axh_mxfp4_expert_gate_up": (st, [vp, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32,
+                                          vp]),
+        "axh_mxfp4_expert_down": (st, [vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, vp]),
+        "axh_expert_plan_bytes": (u64, [u32, u32, u32]),
+        "axh_expert_plan": (st, [vp, vp, vp, u32, u32, u32, vp]),
+        "axh_mxfp4_expert_gate_up_matmul": (st, [vp, vp, vp, vp, vp, vp, vp, vp, u32, vp, vp, u32,
+                                                 u32, u32, u32, u32, vp]),
+        "axh_mxfp4_expert_matmul": (st, [vp, vp, vp, vp, vp, vp, u32, vp, u32, u32, u32, u32, u32,
+                                         vp]),
+        "axh_expert_combine": (st, [vp, u32, vp, vp, vp, vp, u32, u32, u32, u32, vp]),
         "axh_bench_loop": (st, [vp, c.POINTER(_BenchOp), u32, u32, u32, c.POINTER(c.c_float)]),
     }
     for name, (res, args) in sigs.items():
@@ -418,6 +446,41 @@ def q6k_matvec_kernel_name(n_rows: int, sb_per_row: int,
                            variant: Optional[Variant] = None) -> str:
     """Entry point axh_q6k_matvec launches for this shape and variant."""
     return _kernel_name("axh_q6k_matvec_kernel_name", n_rows, sb_per_row, variant)
+
+
+@dataclass(frozen=True)
+class RouteOptions:
+    """How tokens are routed to experts (axh_route_options): `score` "softmax"
+    or "sigmoid"; with n_groups > 1, choices come from the groups_kept groups
+    whose best key (group_best 1), or sum of two best keys (2), is highest;
+    weights are divided by their sum where normalize is set, times scale."""
+
+    n_experts: int
+    top_k: int
+    score: str = "softmax"
+    n_groups: int = 1
+    groups_kept: int = 1
+    group_best: int = 1
+    normalize: bool = True
+    scale: float = 1.0
+
+    def _c(self) -> _RouteOptions:
+        if self.score not in SCORES:
+            raise ValueError(f"unknown score {self.score!r}")
+        return _RouteOptions(self.n_experts, self.top_k, SCORES[self.score], self.n_groups,
+                             self.groups_kept, self.group_best, int(self.normalize), self.scale)
+
+
+def expert_plan_bytes(n_tokens: int, top_k: int, n_experts: int) -> int:
+    """Bytes of the plan that expert_plan writes."""
+    return int(load_library().axh_expert_plan_bytes(n_tokens, top_k, n_experts))
+
+
+def mxfp4_matmul_kernel_name(n_rows: int, cols: int, batch: int, y_type: int = GGML_F32) -> str:
+    """Entry point axh_mxfp4_matmul launches for this shape."""
+    buf = ctypes.create_string_buffer(64)
+    _check(load_library().axh_mxfp4_matmul_kernel_name(n_rows, cols, batch, y_type, buf, 64))
+    return buf.value.decode()
 
 
 def ggml_type_size(ggml_type: int) -> tuple[int, int]:
@@ -875,6 +938,92 @@ class HipContext:
 
     def f16_widen(self, h, f, n: int, stream=None) -> None:
         _check(self._lib.axh_f16_widen(self._raw, _ptr(h), _ptr(f), n, _stream(stream)))
+
+    # ---- MXFP4 and expert layers (include/axh_mx.h) ---------------------------
+    def mxfp4_quantize(self, x, codes, scales, rows: int, cols: int, x_type: int = GGML_F32,
+                       x_stride: int = 0, stream=None) -> None:
+        """codes, scales = MXFP4 of x (rows x cols, x_stride elements between rows)."""
+        _check(self._lib.axh_mxfp4_quantize(self._raw, x_type, _ptr(x), x_stride, _ptr(codes),
+                                            _ptr(scales), rows, cols, _stream(stream)))
+
+    def mxfp4_dequant(self, codes, scales, w, n_blocks: int, w_type: int = GGML_F32,
+                      stream=None) -> None:
+        """w = the 32 * n_blocks values that codes and scales stand for."""
+        _check(self._lib.axh_mxfp4_dequant(self._raw, _ptr(codes), _ptr(scales), w_type, _ptr(w),
+                                           n_blocks, _stream(stream)))
+
+    def mxfp4_unpack_ggml(self, q, codes, scales, n_blocks: int, stream=None) -> None:
+        """codes, scales of n_blocks 17-byte ggml MXFP4 blocks."""
+        _check(self._lib.axh_mxfp4_unpack_ggml(self._raw, _ptr(q), _ptr(codes), _ptr(scales),
+                                               n_blocks, _stream(stream)))
+
+    def mxfp4_matvec(self, codes, scales, x, y, n_rows: int, cols: int, stream=None) -> None:
+        """y = W x, MXFP4 weights and f32 x."""
+        _check(self._lib.axh_mxfp4_matvec(self._raw, _ptr(codes), _ptr(scales), _ptr(x), _ptr(y),
+                                          n_rows, cols, _stream(stream)))
+
+    def mxfp4_matmul(self, w_codes, w_scales, x_codes, x_scales, y, n_rows: int, cols: int,
+                     batch: int, y_type: int = GGML_F32, stream=None) -> None:
+        """y (batch x n_rows) = W X, both MXFP4, on the scaled matrix instructions."""
+        _check(self._lib.axh_mxfp4_matmul(self._raw, _ptr(w_codes), _ptr(w_scales), _ptr(x_codes),
+                                          _ptr(x_scales), y_type, _ptr(y), n_rows, cols, batch,
+                                          _stream(stream)))
+
+    def expert_route(self, logits, bias, experts, weights, n_tokens: int, options: RouteOptions,
+                     logits_type: int = GGML_F32, stream=None) -> None:
+        """experts (int32), weights (f32): n_tokens x top_k choices from router logits;
+        bias: f32 per expert or None."""
+        o = options._c()
+        _check(self._lib.axh_expert_route(self._raw, logits_type, _ptr(logits), _ptr(bias),
+                                          _ptr(experts), _ptr(weights), n_tokens, ctypes.byref(o),
+                                          _stream(stream)))
+
+    def mxfp4_expert_gate_up(self, gate, gate_scales, up, up_scales, x, experts, h, n_rows: int,
+                             cols: int, n_tokens: int, top_k: int, n_experts: int,
+                             stream=None) -> None:
+        """h[slot] = silu(gate[e] x[t]) * (up[e] x[t]) for few tokens, f32 x and h."""
+        _check(self._lib.axh_mxfp4_expert_gate_up(
+            self._raw, _ptr(gate), _ptr(gate_scales), _ptr(up), _ptr(up_scales), _ptr(x),
+            _ptr(experts), _ptr(h), n_rows, cols, n_tokens, top_k, n_experts, _stream(stream)))
+
+    def mxfp4_expert_down(self, codes, scales, h, experts, weights, y, n_rows: int, cols: int,
+                          n_tokens: int, top_k: int, n_experts: int, stream=None) -> None:
+        """y[t] = sum over choices of weight * (W[e] h[slot]) for few tokens, f32 h and y."""
+        _check(self._lib.axh_mxfp4_expert_down(
+            self._raw, _ptr(codes), _ptr(scales), _ptr(h), _ptr(experts), _ptr(weights), _ptr(y),
+            n_rows, cols, n_tokens, top_k, n_experts, _stream(stream)))
+
+    def expert_plan(self, experts, plan, n_tokens: int, top_k: int, n_experts: int,
+                    stream=None) -> None:
+        """plan (expert_plan_bytes) = the slots in order of their experts."""
+        _check(self._lib.axh_expert_plan(self._raw, _ptr(experts), _ptr(plan), n_tokens, top_k,
+                                         n_experts, _stream(stream)))
+
+    def mxfp4_expert_gate_up_matmul(self, gate, gate_scales, up, up_scales, x_codes, x_scales,
+                                    plan, h, h_scales, n_rows: int, cols: int, n_tokens: int,
+                                    top_k: int, n_experts: int, h_type: int = GGML_MXFP4,
+                                    stream=None) -> None:
+        """h[slot] = silu(gate[e] x[t]) * (up[e] x[t]) for prompts, MXFP4 x; h MXFP4 (with
+        h_scales) or f32, f16, bf16."""
+        _check(self._lib.axh_mxfp4_expert_gate_up_matmul(
+            self._raw, _ptr(gate), _ptr(gate_scales), _ptr(up), _ptr(up_scales), _ptr(x_codes),
+            _ptr(x_scales), _ptr(plan), h_type, _ptr(h), _ptr(h_scales), n_rows, cols, n_tokens,
+            top_k, n_experts, _stream(stream)))
+
+    def mxfp4_expert_matmul(self, codes, scales, h_codes, h_scales, plan, y, n_rows: int,
+                            cols: int, n_tokens: int, top_k: int, n_experts: int,
+                            y_type: int = GGML_F32, stream=None) -> None:
+        """y[slot] = W[e] h[slot] for prompts, MXFP4 h (slots x cols)."""
+        _check(self._lib.axh_mxfp4_expert_matmul(
+            self._raw, _ptr(codes), _ptr(scales), _ptr(h_codes), _ptr(h_scales), _ptr(plan),
+            y_type, _ptr(y), n_rows, cols, n_tokens, top_k, n_experts, _stream(stream)))
+
+    def expert_combine(self, slots, experts, weights, y, n_rows: int, n_tokens: int, top_k: int,
+                       y_type: int = GGML_F32, n_experts: int = 0, stream=None) -> None:
+        """y[t] = sum over choices of weight * slots[slot] (slots and y of y_type)."""
+        _check(self._lib.axh_expert_combine(self._raw, y_type, _ptr(slots), _ptr(experts),
+                                            _ptr(weights), _ptr(y), n_rows, n_tokens, top_k,
+                                            n_experts, _stream(stream)))
 
     def cu_count(self) -> int:
         return int(self._lib.axh_cu_count(self._raw))

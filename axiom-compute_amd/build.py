@@ -22,6 +22,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -43,7 +44,7 @@ HIP_FLAGS = [
 # kernarg load before its first memory request.
 KERNEL_FLAGS = ["-mllvm", "-amdgpu-kernarg-preload-count=16"]
 
-KERNELS = ["q4_matvec", "q4_matvec_wide", "q4_matmul"]
+KERNELS = ["q4_matvec", "q4_matvec_wide", "q4_matmul", "mx_elem", "mx_matvec", "mx_matmul"]
 
 # Host-only sanitizer build (g++ lines only).
 SAN_FLAGS = ["-fsanitize=address,undefined", "-fno-omit-frame-pointer",
@@ -62,14 +63,15 @@ def _run(cmd: list[str]) -> None:
 
 def build_kernels() -> dict[str, Path]:
     BUILD.mkdir(exist_ok=True)
-    cos = {}
-    for name in KERNELS:
+    def compile_one(name: str) -> Path:
         src = PKG / "csrc" / "kernels" / f"{name}.hip"
         out = BUILD / f"{name}.co"
         _run([HIPCC, *HIP_FLAGS, *KERNEL_FLAGS, "--offload-device-only", "--no-gpu-bundle-output",
               "-I", str(PKG / "csrc" / "kernels"), "-o", str(out), str(src)])
-        cos[name] = out
-    return cos
+        return out
+
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        return dict(zip(KERNELS, pool.map(compile_one, KERNELS)))
 
 
 def build_runtime(cos: dict[str, Path], sanitize: bool = False) -> Path:
@@ -80,9 +82,7 @@ def build_runtime(cos: dict[str, Path], sanitize: bool = False) -> Path:
     noalloc_o = BUILD / "axh_noalloc.o"
     _run([HIPCC, *HIP_FLAGS, "-fPIC", "-c", "-I", str(ROOT / "include"), "-I", str(rt),
           "-o", str(noalloc_o), str(rt / "axh_noalloc.hip")])
-    _run(["gcc", "-c", f'-DAXH_Q4_MATVEC_CO="{cos["q4_matvec"]}"',
-          f'-DAXH_Q4_MATVEC_WIDE_CO="{cos["q4_matvec_wide"]}"',
-          f'-DAXH_Q4_MATMUL_CO="{cos["q4_matmul"]}"', "-o", str(embed_o),
+    _run(["gcc", "-c", *(f'-DAXH_{n.upper()}_CO="{cos[n]}"' for n in KERNELS), "-o", str(embed_o),
           str(rt / "axh_embed.S")])
     out = SAN_LIB if sanitize else LIB
     out.parent.mkdir(parents=True, exist_ok=True)
@@ -92,7 +92,8 @@ def build_runtime(cos: dict[str, Path], sanitize: bool = False) -> Path:
         *(SAN_FLAGS if sanitize else []),
         "-D__HIP_PLATFORM_AMD__", "-I", str(ROCM / "include"), "-I", str(ROOT / "include"),
         "-I", str(rt),
-        str(rt / "axh_runtime.cpp"), str(rt / "axh_ops.cpp"), str(rt / "axh_gguf.cpp"),
+        str(rt / "axh_runtime.cpp"), str(rt / "axh_ops.cpp"), str(rt / "axh_mx.cpp"),
+        str(rt / "axh_gguf.cpp"),
         str(PKG / "csrc" / "tune" / "axh_tune.cpp"), str(PKG / "csrc" / "tune" / "axh_winners.cpp"),
         str(PKG / "csrc" / "check" / "axh_check.cpp"),
         str(embed_o), str(noalloc_o),

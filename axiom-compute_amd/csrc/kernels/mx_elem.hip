@@ -1,0 +1,498 @@
+// MXFP4 quantisation, decoding and unpacking; routing of tokens to experts,
+// the slots' order by expert, and the weighted sum of the experts' outputs
+// (gfx950).  All of them are bound by memory or, for few tokens, by the
+// latency of a launch.
+#include "mx_common.h"
+
+using namespace axh;
+
+namespace {
+
+// Eight consecutive elements as f32.
+template <class T> __device__ __forceinline__ void load8(const uint8_t *p, float *v);
+template <> __device__ __forceinline__ void load8<TF32>(const uint8_t *p, float *v) {
+  const f32x4_t a = reinterpret_cast<const f32x4_t *>(p)[0];
+  const f32x4_t b = reinterpret_cast<const f32x4_t *>(p)[1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = a[i];
+    v[4 + i] = b[i];
+  }
+}
+template <class T> __device__ __forceinline__ void load8h(const uint8_t *p, float *v) {
+  const u32x4_t w = *reinterpret_cast<const u32x4_t *>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+}
+template <> __device__ __forceinline__ void load8<TF16>(const uint8_t *p, float *v) {
+  load8h<TF16>(p, v);
+}
+template <> __device__ __forceinline__ void load8<TBF16>(const uint8_t *p, float *v) {
+  load8h<TBF16>(p, v);
+}
+
+template <class T> __device__ __forceinline__ void store8(uint8_t *p, const float *v);
+template <> __device__ __forceinline__ void store8<TF32>(uint8_t *p, const float *v) {
+  reinterpret_cast<f32x4_t *>(p)[0] = (f32x4_t){v[0], v[1], v[2], v[3]};
+  reinterpret_cast<f32x4_t *>(p)[1] = (f32x4_t){v[4], v[5], v[6], v[7]};
+}
+template <class T> __device__ __forceinline__ void store8h(uint8_t *p, const float *v) {
+  *reinterpret_cast<u32x4_t *>(p) = (u32x4_t){pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
+                                              pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
+}
+template <> __device__ __forceinline__ void store8<TF16>(uint8_t *p, const float *v) {
+  store8h<TF16>(p, v);
+}
+template <> __device__ __forceinline__ void store8<TBF16>(uint8_t *p, const float *v) {
+  store8h<TBF16>(p, v);
+}
+
+// ---------------------------------------------------------------------------
+// Quantisation.  Four lanes share a block of 32 elements, eight each (one or
+// two 16-byte loads): the block's largest magnitude is a maximum over bit
+// patterns (magnitudes order like integers, NaN above infinity), two DPP steps
+// inside the quad; a power-of-two factor makes the scaling exact, so each
+// element is rounded once.
+// ---------------------------------------------------------------------------
+template <class T>
+__device__ __forceinline__ void quantize_body(const uint8_t *x, uint8_t *codes, uint8_t *scales,
+                                              uint32_t n_blocks, uint32_t row_blocks,
+                                              uint32_t stride_lo, uint32_t stride_hi) {
+  const uint32_t t = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t blk = t >> 2, part = t & 3u;
+  if (blk >= n_blocks) return; // whole quads
+  const uint32_t row = blk / row_blocks;
+  const uint64_t stride = (uint64_t)stride_hi << 32 | stride_lo; // elements
+  const uint64_t at = row * stride + (uint64_t)(blk - row * row_blocks) * 32u + part * 8u;
+  float v[8];
+  load8<T>(x + at * T::kBytes, v);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu;
+    m = b > m ? b : m;
+  }
+  uint32_t o = dpp_u32<kXor1>(m);
+  m = o > m ? o : m;
+  o = dpp_u32<kXor2>(m);
+  m = o > m ? o : m;
+  const uint32_t e = mx_scale_byte(m);
+  const float f = mx_inverse(e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= f;
+  const uint32_t c = e == 255u ? 0u : fp4_pack8(v);
+  reinterpret_cast<uint32_t *>(codes)[(uint64_t)blk * 4u + part] = c;
+  if (part == 0u) scales[blk] = (uint8_t)e;
+}
+
+// ---------------------------------------------------------------------------
+// Decoding: eight codes (one dword) a lane.
+// ---------------------------------------------------------------------------
+template <class T>
+__device__ __forceinline__ void dequant_body(const uint8_t *codes, const uint8_t *scales,
+                                             uint8_t *w, uint32_t n_blocks) {
+  const uint32_t t = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t blk = t >> 2;
+  if (blk >= n_blocks) return;
+  const uint32_t c = reinterpret_cast<const uint32_t *>(codes)[t];
+  const float s = e8m0_to_f32(scales[blk]);
+  float v[8];
+  const f32x2_t p0 = fp4_pair<0>(c), p1 = fp4_pair<1>(c), p2 = fp4_pair<2>(c), p3 = fp4_pair<3>(c);
+  v[0] = p0.x * s;
+  v[1] = p0.y * s;
+  v[2] = p1.x * s;
+  v[3] = p1.y * s;
+  v[4] = p2.x * s;
+  v[5] = p2.y * s;
+  v[6] = p3.x * s;
+  v[7] = p3.y * s;
+  store8<T>(w + (uint64_t)t * 8u * T::kBytes, v);
+}
+
+} // namespace
+
+#define AXH_MX_ELEM(NAME, T)                                                                      \
+  extern "C" __global__ void __launch_bounds__(256) axh_mxfp4_quantize_##NAME(                    \
+      const uint8_t *x, uint8_t *codes, uint8_t *scales, uint32_t n_blocks, uint32_t row_blocks,  \
+      uint32_t stride_lo, uint32_t stride_hi) {                                                   \
+    quantize_body<T>(x, codes, scales, n_blocks, row_blocks, stride_lo, stride_hi);               \
+  }                                                                                               \
+  extern "C" __global__ void __launch_bounds__(256) axh_mxfp4_dequant_##NAME(                     \
+      const uint8_t *codes, const uint8_t *scales, uint8_t *w, uint32_t n_blocks) {               \
+    dequant_body<T>(codes, scales, w, n_blocks);                                                  \
+  }
+AXH_MX_ELEM(f32, TF32)
+AXH_MX_ELEM(f16, TF16)
+AXH_MX_ELEM(bf16, TBF16)
+
+// ggml's MXFP4 blocks (17 bytes: the scale byte, then 16 bytes whose low
+// nibbles are elements 0..15 and whose high nibbles are elements 16..31) as
+// codes and scales.  One lane per output dword (elements 8p .. 8p + 7 of a
+// block): the same nibble of eight consecutive bytes.
+extern "C" __global__ void __launch_bounds__(256) axh_mxfp4_unpack_ggml(const uint8_t *q,
+                                                                       uint8_t *codes,
+                                                                       uint8_t *scales,
+                                                                       uint32_t n_blocks) {
+  const uint32_t t = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t blk = t >> 2, part = t & 3u;
+  if (blk >= n_blocks) return;
+  const uint8_t *b = q + (uint64_t)blk * 17u;
+  const uint32_t shift = (part >> 1) * 4u;
+  uint32_t c = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i) c |= ((b[1u + (part & 1u) * 8u + i] >> shift) & 15u) << (4u * i);
+  reinterpret_cast<uint32_t *>(codes)[t] = c;
+  if (part == 0u) scales[blk] = b[0];
+}
+
+// ---------------------------------------------------------------------------
+// Routing.  One wave per token; lane l holds experts l, l + 64, ... (NPL of
+// them).  Keys are order-preserving unsigned integers, 0 for experts that
+// cannot be chosen, so a round of the top-k is a maximum over the wave (DPP),
+// and the lowest expert among equals is the first set bit of the first
+// non-empty ballot.
+// ---------------------------------------------------------------------------
+namespace {
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  uint32_t o = dpp_u32<kXor1>(v);
+  v = o > v ? o : v;
+  o = dpp_u32<kXor2>(v);
+  v = o > v ? o : v;
+  o = dpp_u32<kHalfMirror>(v);
+  v = o > v ? o : v;
+  o = dpp_u32<kMirror>(v);
+  v = o > v ? o : v;
+  const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 0);
+  const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)v, 16);
+  const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 32);
+  const uint32_t d = (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+  const uint32_t ab = a > b ? a : b, cd = c > d ? c : d;
+  return ab > cd ? ab : cd;
+}
+
+__device__ __forceinline__ float wave_sum_f32(float v) {
+  v += dpp_f32<kXor1>(v);
+  v += dpp_f32<kXor2>(v);
+  v += dpp_f32<kHalfMirror>(v);
+  v += dpp_f32<kMirror>(v);
+  const int i = __builtin_bit_cast(int, v);
+  const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0));
+  const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 16));
+  const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 32));
+  const float d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 48));
+  return (a + b) + (c + d);
+}
+
+// f32 -> unsigned with the same order; -0 counts as +0, NaN as -inf.
+__device__ __forceinline__ uint32_t order_of(float f) {
+  if (f != f) f = -__builtin_inff();
+  const uint32_t b = __builtin_bit_cast(uint32_t, f + 0.0f);
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+  return __builtin_bit_cast(float, (o >> 31) ? o & 0x7FFFFFFFu : ~o);
+}
+constexpr uint32_t kOrderMinusInf = 0x007FFFFFu; // order_of(-inf)
+
+enum : uint32_t { kSigmoid = 1u, kNormalize = 2u, kKeyIsLogit = 4u };
+
+// Logit i of a token, whatever their type.
+template <class T> __device__ __forceinline__ float logit_at(const uint8_t *row, uint32_t i);
+template <> __device__ __forceinline__ float logit_at<TF32>(const uint8_t *row, uint32_t i) {
+  return reinterpret_cast<const float *>(row)[i];
+}
+template <> __device__ __forceinline__ float logit_at<TF16>(const uint8_t *row, uint32_t i) {
+  return (float)reinterpret_cast<const _Float16 *>(row)[i];
+}
+template <> __device__ __forceinline__ float logit_at<TBF16>(const uint8_t *row, uint32_t i) {
+  return __builtin_bit_cast(float, (uint32_t)reinterpret_cast<const uint16_t *>(row)[i] << 16);
+}
+
+template <class T, int NPL>
+__device__ __forceinline__ void route_body(const uint8_t *logits, const float *bias,
+                                           int32_t *experts, float *weights, uint32_t n_tokens,
+                                           uint32_t n_experts, uint32_t top_k, uint32_t flags,
+                                           uint32_t n_groups, uint32_t groups_kept,
+                                           uint32_t group_best, float scale, uint32_t *lds) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t token = blockIdx.x * 4u + wave;
+  const bool real = token < n_tokens; // waves past the end only keep barriers company
+  const uint8_t *row = logits + (uint64_t)(real ? token : 0u) * n_experts * T::kBytes;
+  const float kInf = __builtin_inff();
+
+  float l[NPL]; // logits, -inf where masked, NaN or past the end
+  float most = -kInf;
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    const uint32_t e = 64u * j + lane;
+    const float v = e < n_experts ? logit_at<T>(row, e) : -kInf;
+    l[j] = v == v ? v : -kInf;
+    most = l[j] > most ? l[j] : most;
+  }
+  float s[NPL]; // scores; masked experts score 0
+  if (flags & kSigmoid) {
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) s[j] = 1.0f / (1.0f + expf(-l[j]));
+  } else {
+    most = value_of(wave_max_u32(order_of(most)));
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) { // +inf logits share all the weight
+      s[j] = l[j] == -kInf ? 0.0f : l[j] == most ? 1.0f : expf(l[j] - most);
+      sum += s[j];
+    }
+    sum = wave_sum_f32(sum);
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) s[j] = sum > 0.0f ? s[j] / sum : 0.0f;
+  }
+  uint32_t key[NPL];
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    const uint32_t e = 64u * j + lane;
+    float k = (flags & kKeyIsLogit) ? l[j] : s[j];
+    if (bias) k += e < n_experts ? bias[e] : 0.0f;
+    const uint32_t o = order_of(k);
+    key[j] = l[j] == -kInf || o <= kOrderMinusInf ? 0u : o;
+  }
+
+  if (n_groups > 1u) {
+    // Every lane looks at its part of one group: 64 / G lanes (a power of two)
+    // per group, then the two best of the lanes of a group are merged.
+    uint32_t *mine = lds + wave * (64u * NPL + 64u);
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) mine[64u * j + lane] = key[j];
+    __syncthreads();
+    const uint32_t per = n_experts / n_groups;
+    uint32_t log_lanes = 0;
+    while ((n_groups << (log_lanes + 1u)) <= 64u) ++log_lanes;
+    const uint32_t lanes = 1u << log_lanes, g = lane >> log_lanes, part = lane & (lanes - 1u);
+    uint32_t a = 0, b = 0; // best and second best
+    if (g < n_groups)
+      for (uint32_t i = part; i < per; i += lanes) {
+        const uint32_t k = mine[g * per + i];
+        b = k > a ? a : k > b ? k : b;
+        a = k > a ? k : a;
+      }
+    for (uint32_t m = 1; m < lanes; m <<= 1) {
+      const uint32_t oa = (uint32_t)__shfl_xor((int)a, (int)m);
+      const uint32_t ob = (uint32_t)__shfl_xor((int)b, (int)m);
+      const uint32_t lo = a < oa ? a : oa;
+      a = a < oa ? oa : a;
+      b = b < ob ? ob : b;
+      b = b < lo ? lo : b;
+    }
+    uint32_t gk = a;
+    if (group_best == 2u)
+      gk = order_of((a ? value_of(a) : -kInf) + (b ? value_of(b) : -kInf));
+    uint32_t *gkeys = mine + 64u * NPL;
+    if (g < n_groups && part == 0u) gkeys[g] = gk;
+    __syncthreads();
+    uint32_t rank = 0; // of group `lane`: greater ones and equal ones before it
+    const uint32_t own = lane < n_groups ? gkeys[lane] : 0u;
+    for (uint32_t i = 0; i < n_groups; ++i) {
+      const uint32_t k = gkeys[i];
+      rank += k > own || (k == own && i < lane) ? 1u : 0u;
+    }
+    const uint64_t kept = __ballot(lane < n_groups && rank < groups_kept);
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) {
+      const uint32_t e = 64u * j + lane;
+      if (e < n_experts && !((kept >> (e / per)) & 1u)) key[j] = 0u;
+    }
+  }
+
+  int32_t picked = -1; // lane i holds choice i of up to 64
+  float weight = 0.0f;
+  for (uint32_t i = 0; i < top_k; ++i) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) best = key[j] > best ? key[j] : best;
+    best = wave_max_u32(best);
+    if (best == 0u) break; // nothing left: -1 and weight 0
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) {
+      const uint64_t at = __ballot(key[j] == best);
+      if (!found && at) {
+        found = true;
+        const int who = __builtin_ctzll(at);
+        const float w = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s[j]), who));
+        if (lane == i) {
+          picked = 64 * j + who;
+          weight = w;
+        }
+        if (lane == (uint32_t)who) key[j] = 0u;
+      }
+    }
+  }
+  if (flags & kNormalize) {
+    const float sum = wave_sum_f32(weight);
+    weight = sum > 0.0f ? weight / sum : 0.0f;
+  }
+  if (real && lane < top_k) {
+    experts[(uint64_t)token * top_k + lane] = picked;
+    weights[(uint64_t)token * top_k + lane] = weight * scale;
+  }
+}
+
+} // namespace
+
+#define AXH_ROUTE(NAME, T, NPL)                                                                   \
+  extern "C" __global__ void __launch_bounds__(256) axh_expert_route_##NAME##_n##NPL(             \
+      const uint8_t *logits, const float *bias, int32_t *experts, float *weights,                 \
+      uint32_t n_tokens, uint32_t n_experts, uint32_t top_k, uint32_t flags, uint32_t n_groups,   \
+      uint32_t groups_kept, uint32_t group_best, uint32_t scale) {                                \
+    __shared__ uint32_t lds[4 * (64 * NPL + 64)];                                                 \
+    route_body<T, NPL>(logits, bias, experts, weights, n_tokens, n_experts, top_k, flags,         \
+                       n_groups, groups_kept, group_best, __builtin_bit_cast(float, scale), lds); \
+  }
+#define AXH_ROUTE_N(NPL)   \
+  AXH_ROUTE(f32, TF32, NPL) \
+  AXH_ROUTE(f16, TF16, NPL) \
+  AXH_ROUTE(bf16, TBF16, NPL)
+AXH_ROUTE_N(1)
+AXH_ROUTE_N(2)
+AXH_ROUTE_N(4)
+AXH_ROUTE_N(8)
+AXH_ROUTE_N(16)
+
+// ---------------------------------------------------------------------------
+// The order of slots by expert: a stable counting sort in one workgroup.  Slot
+// i is choice i % top_k of token i / top_k.  Wave w takes a contiguous part of
+// the slots; counts per wave and expert, their prefix sums over (expert, wave),
+// then each wave hands out places in slot order: within 64 slots, the lanes
+// with the same expert are found by one ballot per bit of the expert's index.
+// plan: offsets[n_experts + 1], padded to 16 words, then the slots.
+// ---------------------------------------------------------------------------
+extern "C" __global__ void __launch_bounds__(1024) axh_expert_plan(const int32_t *experts,
+                                                                  uint32_t *plan,
+                                                                  uint32_t n_slots,
+                                                                  uint32_t n_experts,
+                                                                  uint32_t id_bits) {
+  extern __shared__ uint32_t lds[]; // [16][n_experts] counts, then places; [16] sums
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  uint32_t *sums = lds + 16u * n_experts;
+  for (uint32_t i = tid; i < 16u * n_experts; i += 1024u) lds[i] = 0u;
+  __syncthreads();
+  // a wave's part is a multiple of 64, so only the last 64 are partial
+  const uint32_t part = ((n_slots + 1023u) / 1024u) * 64u;
+  const uint32_t from = wave * part;
+  const uint32_t to = from + part < n_slots ? from + part : n_slots;
+  for (uint32_t i = from + lane; i < to; i += 64u) {
+    const uint32_t e = (uint32_t)experts[i];
+    if (e < n_experts) atomicAdd(&lds[wave * n_experts + e], 1u);
+  }
+  __syncthreads();
+  // thread e: the expert's total, and its waves' counts turned into prefixes
+  uint32_t total = 0;
+  if (tid < n_experts)
+    for (uint32_t w = 0; w < 16u; ++w) {
+      const uint32_t c = lds[w * n_experts + tid];
+      lds[w * n_experts + tid] = total;
+      total += c;
+    }
+  uint32_t incl = total; // inclusive prefix over the experts of this wave
+#pragma unroll
+  for (uint32_t d = 1; d < 64u; d <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)incl, d);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 63u) sums[wave] = incl;
+  __syncthreads();
+  uint32_t base = 0;
+  for (uint32_t w = 0; w < wave; ++w) base += sums[w];
+  const uint32_t first = base + incl - total;
+  if (tid < n_experts) {
+    plan[tid] = first;
+    if (tid == n_experts - 1u) plan[n_experts] = first + total;
+    for (uint32_t w = 0; w < 16u; ++w) lds[w * n_experts + tid] += first;
+  }
+  __syncthreads();
+  uint32_t *order = plan + ((n_experts + 1u + 15u) & ~15u);
+  for (uint32_t i0 = from; i0 < to; i0 += 64u) {
+    const uint32_t i = i0 + lane;
+    const uint32_t e = i < to ? (uint32_t)experts[i] : 0xFFFFFFFFu;
+    const bool in = e < n_experts;
+    uint64_t same = __ballot(in);
+    for (uint32_t b = 0; b < id_bits; ++b) {
+      const bool bit = (e >> b) & 1u;
+      const uint64_t set = __ballot(bit);
+      same &= bit ? set : ~set;
+    }
+    if (in) {
+      const uint32_t before = __builtin_popcountll(same & ((1ull << lane) - 1ull));
+      const uint32_t at = lds[wave * n_experts + e];
+      order[at + before] = i;
+      // the last of the lanes moves the place on; the wave's LDS operations are in order
+      if ((same >> lane) == 1ull) lds[wave * n_experts + e] = at + before + 1u;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// y[t] = sum over a token's choices of weight * slot output, in f32, rounded
+// once.  Choices outside 0 .. n_experts - 1 (the router's -1 among them) are left
+// out: their slots hold nothing.  Eight columns a lane where n_cols is a multiple of
+// eight and the rows are 16-byte aligned, else one.
+// ---------------------------------------------------------------------------
+namespace {
+
+template <class T> __device__ __forceinline__ void store1(uint8_t *p, float v);
+template <> __device__ __forceinline__ void store1<TF32>(uint8_t *p, float v) {
+  *reinterpret_cast<float *>(p) = v;
+}
+template <> __device__ __forceinline__ void store1<TF16>(uint8_t *p, float v) {
+  *reinterpret_cast<uint16_t *>(p) = (uint16_t)pack2<TF16>(v, 0.0f);
+}
+template <> __device__ __forceinline__ void store1<TBF16>(uint8_t *p, float v) {
+  *reinterpret_cast<uint16_t *>(p) = (uint16_t)pack2<TBF16>(v, 0.0f);
+}
+
+template <class T>
+__device__ __forceinline__ void combine_body(const uint8_t *slots, const int32_t *experts,
+                                             const float *weights, uint8_t *y, uint32_t n_cols,
+                                             uint32_t top_k, uint32_t n_experts) {
+  const uint32_t token = blockIdx.x;
+  const uint64_t first = (uint64_t)token * top_k;
+  if (n_cols % 8u == 0u) {
+    const uint32_t c = (blockIdx.y * 256u + threadIdx.x) * 8u;
+    if (c >= n_cols) return;
+    float acc[8] = {};
+    for (uint32_t k = 0; k < top_k; ++k) {
+      if ((uint32_t)experts[first + k] >= n_experts) continue;
+      const float w = weights[first + k];
+      float v[8];
+      load8<T>(slots + ((first + k) * n_cols + c) * T::kBytes, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
+    }
+    store8<T>(y + ((uint64_t)token * n_cols + c) * T::kBytes, acc);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t c = blockIdx.y * 2048u + i * 256u + threadIdx.x;
+      if (c >= n_cols) return;
+      float acc = 0.0f;
+      for (uint32_t k = 0; k < top_k; ++k) {
+        if ((uint32_t)experts[first + k] >= n_experts) continue;
+        const uint8_t *row = slots + (first + k) * n_cols * T::kBytes;
+        acc = __builtin_fmaf(weights[first + k], logit_at<T>(row, c), acc);
+      }
+      store1<T>(y + ((uint64_t)token * n_cols + c) * T::kBytes, acc);
+    }
+  }
+}
+
+} // namespace
+
+#define AXH_COMBINE(NAME, T)                                                                      \
+  extern "C" __global__ void __launch_bounds__(256) axh_expert_combine_##NAME(                    \
+      const uint8_t *slots, const int32_t *experts, const float *weights, uint8_t *y,             \
+      uint32_t n_cols, uint32_t top_k, uint32_t n_experts) {                                      \
+    combine_body<T>(slots, experts, weights, y, n_cols, top_k, n_experts);                        \
+  }
+AXH_COMBINE(f32, TF32)
+AXH_COMBINE(f16, TF16)
+AXH_COMBINE(bf16, TBF16)

@@ -27,6 +27,7 @@
 #include <vector>
 
 #include "axh_gguf.h"
+#include "axh_mx.h"
 #include "axh_internal.h"
 
 using axh::fail;
@@ -70,6 +71,7 @@ TypeSize type_size(uint32_t t) {
   case AXH_GGML_I64: return {1, 8};
   case AXH_GGML_F64: return {1, 8};
   case AXH_GGML_BF16: return {1, 2};
+  case AXH_GGML_MXFP4: return {32, 17};
   default: return {0, 0};
   }
 }

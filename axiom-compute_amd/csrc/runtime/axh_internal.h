@@ -121,6 +121,11 @@ bool is_builtin_code_object(const void *co, size_t bytes);
 // Builtin kernel by entry name, prepared once per context.
 axh_status builtin_kernel(axh_context *ctx, const char *entry, uint32_t n_buffers,
                           uint32_t pc_bytes, uint32_t wg_x, axh_kernel **out);
+// The code objects of the MXFP4 and expert kernels (axh_mx.cpp), by number, and
+// a kernel of one of them by entry name, prepared once per context.
+bool mx_code_object(uint32_t i, const void **co, size_t *bytes);
+axh_status mx_kernel(axh_context *ctx, uint32_t object, const char *entry, uint32_t n_buffers,
+                     uint32_t pc_bytes, uint32_t wg_x, axh_kernel **out);
 hipStream_t pick_stream(axh_context *ctx, void *stream);
 // Set-up of the allocation-free matvec (axh_noalloc.hip): resolves this
 // device's scratch array and prepares its kernel.  Run by axh_context_create.

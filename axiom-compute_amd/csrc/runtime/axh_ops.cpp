@@ -138,6 +138,10 @@ bool is_builtin_code_object(const void *co, size_t bytes) {
     const size_t n = (size_t)(o[1] - o[0]);
     if (bytes == n && (co == o[0] || std::memcmp(co, o[0], n) == 0)) return true;
   }
+  const void *mx = nullptr;
+  size_t n = 0;
+  for (uint32_t i = 0; mx_code_object(i, &mx, &n); ++i)
+    if (bytes == n && (co == mx || std::memcmp(co, mx, n) == 0)) return true;
   return false;
 }
 

@@ -24,7 +24,7 @@ _SCALAR = {U8: "<B", I8: "<b", U16: "<H", I16: "<h", U32: "<I", I32: "<i", F32: 
 # ggml tensor types (GGUF ids)
 GGML_F32, GGML_F16, GGML_Q4_0 = 0, 1, 2
 GGML_Q4_K, GGML_Q5_K, GGML_Q6_K = 12, 13, 14
-GGML_BF16 = 30
+GGML_BF16, GGML_MXFP4 = 30, 39
 
 
 @dataclass(frozen=True)
