@@ -9,12 +9,11 @@
 // scales are exact in f32.
 //
 // Two kinds of kernel:
-//   * skinny (few columns, bound by W's bytes): a workgroup has one 32-row tile
-//     of W (gate/up: one of each matrix), its waves split the K axis, operands
-//     go straight to registers and the waves' partial tiles meet in LDS;
-//   * tile (many columns, bound by the matrix cores): a workgroup has a BM x BN
-//     tile, K in steps of 256 through two LDS buffers filled by direct-to-LDS
-//     loads, each wave a part of the tile.
+//   * K-split (few columns and rows, bound by the time that W's bytes take to
+//     come): a workgroup has 16 or 32 rows of W (gate/up: 32 of each matrix) and
+//     32 columns, its waves split the K axis;
+//   * tile: a workgroup has a BM x BN tile, each wave a part of it, and all its
+//     waves go through K together.
 #include "mx_common.h"
 
 #include <type_traits>
@@ -38,6 +37,14 @@ __device__ __forceinline__ f32x16_t mfma(u32x4_t a, u32x4_t b, f32x16_t c, uint3
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, kk, (int)sa, kk, (int)sb);
 }
 
+template <int kk>
+__device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c, uint32_t sa,
+                                          uint32_t sb) {
+  const i32x8_t A = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+  const i32x8_t B = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, kk, (int)sa, kk, (int)sb);
+}
+
 // The eight scale bytes of a row's K step (blocks 8s .. 8s + 7), as loaded:
 // rows of at least eight blocks are read inside the row, the bytes of a last,
 // partial step shifted down at their use (scales8); the scales past the row's
@@ -51,9 +58,11 @@ __device__ __forceinline__ ScaleStep scale_step(uint32_t s, uint32_t nblk) {
   const uint32_t at = want < last ? want : last;
   return {at, nblk < 8u ? 0u : (want - at) * 8u};
 }
+template <bool kShort>
 __device__ __forceinline__ u32x2_t load_scales8(__amdgpu_buffer_rsrc_t r, uint32_t row_off,
                                                 ScaleStep st, uint32_t nblk) {
-  if (nblk >= 8u) return __builtin_amdgcn_raw_buffer_load_b64(r, (int)(row_off + st.at), 0, 0);
+  if constexpr (!kShort)
+    return __builtin_amdgcn_raw_buffer_load_b64(r, (int)(row_off + st.at), 0, 0);
   uint32_t v[8];
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i)
@@ -70,11 +79,17 @@ __device__ __forceinline__ uint32_t scale_selector(uint32_t half) {
   return half ? 0x07050301u : 0x06040200u;
 }
 
-// Four consecutive rows of one output column.
+// Four consecutive rows of one output column; kVec: n_rows and y allow whole
+// vector stores (store_whole), so the four are all there or none.
 template <class T>
+__device__ __forceinline__ bool store_whole(const uint8_t *y, uint32_t n_rows) {
+  return n_rows % 4u == 0u && ((uintptr_t)y & (4u * T::kBytes - 1u)) == 0u;
+}
+template <class T, bool kVec>
 __device__ __forceinline__ void store4(uint8_t *col, uint32_t r, uint32_t n_rows, f32x4_t v) {
   uint8_t *p = col + (uint64_t)r * T::kBytes;
-  if (r + 4u <= n_rows && ((uintptr_t)p & (4u * T::kBytes - 1u)) == 0u) {
+  if constexpr (kVec) {
+    if (r >= n_rows) return;
     if constexpr (T::kBytes == 4)
       *reinterpret_cast<f32x4_t *>(p) = v;
     else
@@ -91,7 +106,6 @@ __device__ __forceinline__ void store4(uint8_t *col, uint32_t r, uint32_t n_rows
       }
   }
 }
-
 
 // A 32-feature block of one column of h as MXFP4: lanes l and l + 32 of a wave
 // hold its features 8q + 4 (lane / 32) + i in h[4q + i].  Each lane packs its
@@ -152,7 +166,7 @@ struct Tile {
 // Workgroup -> tile.  Consecutive workgroups go to the eight XCDs in turn; each
 // XCD is given a contiguous part of the tiles, rows fastest for expert layers
 // (the tiles of one group of columns share X), columns fastest otherwise.
-template <Mode M, int BN> __device__ __forceinline__ Tile tile_of(const Args &a, uint32_t *lds) {
+template <Mode M, int BN> __device__ __forceinline__ Tile tile_of(const Args &a) {
   const uint32_t total = gridDim.x, id = blockIdx.x;
   const uint32_t per = total / 8u, rest = total % 8u, xcd = id % 8u;
   const uint32_t t = xcd * per + (xcd < rest ? xcd : rest) + id / 8u;
@@ -202,7 +216,6 @@ template <Mode M, int BN> __device__ __forceinline__ Tile tile_of(const Args &a,
     }
   }
   if (r.count > (uint32_t)BN) r.count = BN;
-  (void)lds;
   return r;
 }
 
@@ -211,190 +224,37 @@ __device__ __forceinline__ const uint32_t *plan_order(const Args &a) {
 }
 
 // Finishes four rows r .. r + 3 of a column (not packed).
-template <Mode M, class T>
+template <Mode M, class T, bool kVec>
 __device__ __forceinline__ void emit4(const Args &a, uint32_t out_row, uint32_t r, f32x4_t g,
                                       f32x4_t u) {
   if constexpr (M == kGateUp) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) g[i] = swiglu(g[i], u[i]);
   }
-  if (r < a.n_rows)
-    store4<T>(a.y + (uint64_t)out_row * a.n_rows * T::kBytes, r, a.n_rows, g);
+  store4<T, kVec>(a.y + (uint64_t)out_row * a.n_rows * T::kBytes, r, a.n_rows, g);
 }
 
 // ---------------------------------------------------------------------------
-// Skinny kind: NW waves, 32 rows (of one matrix, or of gate and up), 32 * NI
-// columns.
+// K-split kind: 32 or 16 rows (gate/up: 32 of each matrix) by 32 columns, NW
+// waves.  Steps of 256 along K go to the waves in turn; each wave fills NB
+// buffers of its own in LDS by direct-to-LDS loads, so nothing but its load
+// counter is waited for until the waves' partial tiles are summed in LDS, in
+// the waves' order.  The LDS rows are the tile kind's.
 // ---------------------------------------------------------------------------
-template <Mode M, class T, bool kPacked, int NI, int NW>
-__device__ __forceinline__ void skinny_body(const Args &a, f32x4_t *lds) {
+template <Mode M, class T, bool kPacked, int kRows, int NW, int NB>
+__device__ __forceinline__ void ksplit_body(const Args &a, uint8_t *lds) {
   constexpr int MI = M == kGateUp ? 2 : 1;
-  constexpr int BN = 32 * NI;
+  constexpr uint32_t kARows = MI * kRows, kBuf = (kARows + 32u) * 128u;
+  constexpr int kALoads = kARows / 8, kLoads = kALoads + 4;
+  static_assert(kRows == 32 || (kRows == 16 && M != kGateUp), "16 rows: one matrix");
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t half = lane >> 5, r32 = lane & 31u;
-  const Tile t = tile_of<M, BN>(a, nullptr);
-  if (!t.real) return;
-  const uint32_t row0 = t.m * 32u;
-  const uint32_t nblk = a.nblk, row_bytes = nblk * 16u;
-  const uint64_t matrix = (uint64_t)a.n_rows * nblk, wat = t.expert * matrix + (uint64_t)row0 * nblk;
-  const uint32_t rows = a.n_rows - row0 < 32u ? a.n_rows - row0 : 32u;
-  __amdgpu_buffer_rsrc_t wc[MI], ws[MI];
-  wc[0] = rsrc(a.wc + wat * 16u, rows * row_bytes);
-  ws[0] = rsrc(a.ws + wat, rows * nblk);
-  if constexpr (MI == 2) {
-    wc[1] = rsrc(a.uc + wat * 16u, rows * row_bytes);
-    ws[1] = rsrc(a.us + wat, rows * nblk);
-  }
-  // columns: X's rows, and the rows of y they go to
-  uint32_t xrow[NI], out[NI];
-  uint64_t xbase = 0;
-  uint32_t xrows = a.n_x;
-  if constexpr (M == kDense) {
-    xbase = t.n0;
-    xrows = t.count;
-  }
-#pragma unroll
-  for (int n = 0; n < NI; ++n) {
-    const uint32_t j = 32u * n + r32;
-    if constexpr (M == kDense) {
-      xrow[n] = j < t.count ? j : 0xFFFFFFFFu;
-      out[n] = t.n0 + j;
-    } else {
-      const uint32_t slot = plan_order(a)[t.first + (j < t.count ? j : 0u)];
-      xrow[n] = j < t.count ? slot / a.x_div : 0xFFFFFFFFu;
-      out[n] = slot;
-    }
-  }
-  const __amdgpu_buffer_rsrc_t xc = rsrc(a.xc + xbase * row_bytes, xrows * row_bytes);
-  const __amdgpu_buffer_rsrc_t xs = rsrc(a.xs + xbase * nblk, xrows * nblk);
-
-  f32x16_t acc[MI][NI] = {};
-  const uint32_t sel = scale_selector(half);
-  const uint32_t steps = (nblk + 7u) / 8u;
-  struct Step {
-    u32x4_t a[MI][4], b[NI][4];
-    u32x2_t sa[MI], sb[NI];
-    ScaleStep st;
-  };
-  auto load = [&](uint32_t s, Step &p) {
-    p.st = scale_step(s, nblk);
-#pragma unroll
-    for (int m = 0; m < MI; ++m) p.sa[m] = load_scales8(ws[m], r32 * nblk, p.st, nblk);
-#pragma unroll
-    for (int n = 0; n < NI; ++n)
-      p.sb[n] = load_scales8(xs, xrow[n] == 0xFFFFFFFFu ? kFar : xrow[n] * nblk, p.st, nblk);
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) {
-      const uint32_t blk = 8u * s + 2u * k + half;
-      const bool in = blk < nblk;
-#pragma unroll
-      for (int m = 0; m < MI; ++m)
-        p.a[m][k] = __builtin_amdgcn_raw_buffer_load_b128(
-            wc[m], (int)(in ? r32 * row_bytes + blk * 16u : kFar), 0, 0);
-#pragma unroll
-      for (int n = 0; n < NI; ++n)
-        p.b[n][k] = __builtin_amdgcn_raw_buffer_load_b128(
-            xc, (int)(in && xrow[n] != 0xFFFFFFFFu ? xrow[n] * row_bytes + blk * 16u : kFar), 0,
-            0);
-    }
-  };
-  auto multiply = [&](const Step &p) {
-    uint32_t sa[MI], sb[NI];
-#pragma unroll
-    for (int m = 0; m < MI; ++m) sa[m] = lane_scales(p.sa[m], p.st, sel);
-#pragma unroll
-    for (int n = 0; n < NI; ++n) sb[n] = lane_scales(p.sb[n], p.st, sel);
-#pragma unroll
-    for (int m = 0; m < MI; ++m)
-#pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        acc[m][n] = mfma<0>(p.a[m][0], p.b[n][0], acc[m][n], sa[m], sb[n]);
-        acc[m][n] = mfma<1>(p.a[m][1], p.b[n][1], acc[m][n], sa[m], sb[n]);
-        acc[m][n] = mfma<2>(p.a[m][2], p.b[n][2], acc[m][n], sa[m], sb[n]);
-        acc[m][n] = mfma<3>(p.a[m][3], p.b[n][3], acc[m][n], sa[m], sb[n]);
-      }
-  };
-  Step p0, p1;
-  uint32_t s = wave;
-  if (s < steps) load(s, p0);
-  for (; s < steps; s += 2u * NW) {
-    if (s + NW < steps) load(s + NW, p1);
-    multiply(p0);
-    if (s + 2u * NW < steps) load(s + 2u * NW, p0);
-    if (s + NW < steps) multiply(p1);
-  }
-
-  // partial tiles: [wave][matrix][column group][quarter][lane]
-  constexpr uint32_t kTiles = MI * NI;
-#pragma unroll
-  for (int m = 0; m < MI; ++m)
-#pragma unroll
-    for (int n = 0; n < NI; ++n)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        lds[((wave * kTiles + m * NI + n) * 4u + q) * 64u + lane] =
-            (f32x4_t){acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2],
-                      acc[m][n][4 * q + 3]};
-  __syncthreads();
-  auto total = [&](uint32_t m, uint32_t n, uint32_t q) {
-    f32x4_t v = lds[((m * NI + n) * 4u + q) * 64u + lane];
-#pragma unroll
-    for (uint32_t w = 1; w < NW; ++w) v += lds[((w * kTiles + m * NI + n) * 4u + q) * 64u + lane];
-    return v;
-  };
-  if constexpr (kPacked) {
-    for (uint32_t n = wave; n < (uint32_t)NI; n += NW) {
-      float h[16];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4_t g = total(0, n, q), u = total(MI - 1, n, q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[4 * q + i] = swiglu(g[i], u[i]);
-      }
-      uint32_t o = out[0];
-#pragma unroll
-      for (uint32_t k = 1; k < NI; ++k) o = n == k ? out[k] : o;
-      store_packed(a.y, a.ysc, (uint64_t)o * (a.n_rows / 32u) + t.m, h, half,
-                   32u * n + r32 < t.count);
-    }
-  } else {
-    for (uint32_t i = wave; i < 4u * NI; i += NW) {
-      const uint32_t n = i / 4u, q = i % 4u;
-      const f32x4_t g = total(0, n, q), u = M == kGateUp ? total(MI - 1, n, q) : g;
-      uint32_t o = out[0];
-#pragma unroll
-      for (uint32_t k = 1; k < NI; ++k) o = n == k ? out[k] : o;
-      if (32u * n + r32 < t.count) emit4<M, T>(a, o, row0 + 8u * q + 4u * half, g, u);
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Tile kind: BM x BN outputs (gate/up: BM / 2 rows of each matrix, in turns of
-// 32), WM x WN waves.  An LDS row is 128 bytes, the codes of one K step, with
-// 16-byte piece c at place c ^ (row % 8): the 32 rows that a fragment read
-// touches then meet all the banks.
-// ---------------------------------------------------------------------------
-template <Mode M, class T, bool kPacked, int BM, int BN, int WM, int WN>
-__device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
-  constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
-  constexpr uint32_t kBuf = (BM + BN) * 128u;
-  constexpr int kLoads = (BM + BN) / 8 / NW; // per wave and step; rows of A first
-  constexpr int kALoads = BM / 8 / NW;
-  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads per wave");
-  static_assert(M != kGateUp || MI % 2 == 0, "gate and up rows in one wave");
-  constexpr uint32_t kRows = M == kGateUp ? BM / 2 : BM; // rows of y
-  const uint32_t lane = threadIdx.x & 63u;
-  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t wm = wave / WN, wn = wave % WN;
-  const uint32_t half = lane >> 5, r32 = lane & 31u;
-  const Tile t = tile_of<M, BN>(a, nullptr);
+  const Tile t = tile_of<M, 32>(a);
   if (!t.real) return;
   const uint32_t row0 = t.m * kRows;
   const uint32_t nblk = a.nblk, row_bytes = nblk * 16u;
-  const uint64_t wat = (uint64_t)t.expert * a.n_rows * nblk + (uint64_t)row0 * nblk;
-  const uint32_t rows = a.n_rows - row0 < kRows ? a.n_rows - row0 : kRows;
+  const uint64_t wat = ((uint64_t)t.expert * a.n_rows + row0) * nblk;
+  const uint32_t rows = a.n_rows - row0 < (uint32_t)kRows ? a.n_rows - row0 : (uint32_t)kRows;
   const __amdgpu_buffer_rsrc_t wc = rsrc(a.wc + wat * 16u, rows * row_bytes);
   const __amdgpu_buffer_rsrc_t ws = rsrc(a.ws + wat, rows * nblk);
   const __amdgpu_buffer_rsrc_t uc = M == kGateUp ? rsrc(a.uc + wat * 16u, rows * row_bytes) : wc;
@@ -403,14 +263,246 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   const uint32_t xrows = M == kDense ? t.count : a.n_x;
   const __amdgpu_buffer_rsrc_t xc = rsrc(a.xc + xbase * row_bytes, xrows * row_bytes);
   const __amdgpu_buffer_rsrc_t xs = rsrc(a.xs + xbase * nblk, xrows * nblk);
+  auto slot_of = [&](uint32_t j) {
+    return M == kDense ? t.n0 + j : plan_order(a)[t.first + (j < t.count ? j : 0u)];
+  };
+  auto xrow_of = [&](uint32_t j) { return M == kDense ? j : slot_of(j) / a.x_div; };
+
+  // this lane's part of each load of codes: row 8 * load + lane / 8 of A or of B
+  const uint32_t l8 = lane >> 3;
+  uint32_t off[kLoads], piece[2]; // the piece depends on the row mod 16
+#pragma unroll
+  for (uint32_t p = 0; p < 2; ++p) piece[p] = (lane & 7u) ^ ((4u * p + (l8 >> 1)) & 7u);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    if (i < kALoads) {
+      off[i] = ((8u * i + l8) % kRows) * row_bytes + piece[i & 1] * 16u;
+    } else {
+      const uint32_t j = 8u * (i - kALoads) + l8;
+      off[i] = j < t.count ? xrow_of(j) * row_bytes + piece[i & 1] * 16u : kFar;
+    }
+  }
+  // the lane's rows of scales
+  const uint32_t r32 = lane & 31u, group = kRows == 32 ? lane >> 5 : lane >> 4;
+  const uint32_t arow = (lane & (kRows - 1u)) * nblk;
+  uint32_t brow[kRows == 32 ? 1 : 2];
+#pragma unroll
+  for (uint32_t n = 0; n < (kRows == 32 ? 1u : 2u); ++n) {
+    const uint32_t j = kRows == 32 ? r32 : 16u * n + (lane & 15u);
+    brow[n] = j < t.count ? xrow_of(j) * nblk : kFar;
+  }
+  constexpr int NI = kRows == 32 ? 1 : 2; // operand tiles of B
+  const uint32_t sel = kRows == 32 ? scale_selector(group) : group | (group + 4u) << 8;
+
+  uint8_t *const ring = lds + wave * (NB * kBuf);
+  const uint32_t steps = (nblk + 7u) / 8u;
+  struct Scales {
+    u32x2_t a[MI], b[NI];
+  };
+  auto request = [&](uint32_t s, uint32_t buf) { // steps past the end: zeros
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const bool in = 8u * s + piece[i & 1] < nblk;
+      const bool up = M == kGateUp && i >= kRows / 8 && i < kALoads;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kALoads ? (up ? uc : wc) : xc,
+                                               (lds_void_t *)(ring + buf * kBuf + i * 1024u), 16,
+                                               (int)(in ? off[i] + s * 128u : kFar), 0, 0, 0);
+    }
+  };
+  auto load_scales = [&](uint32_t s, Scales &c, auto few) {
+    constexpr bool kFew = decltype(few)::value;
+    const ScaleStep st = scale_step(s < steps ? s : steps - 1u, nblk);
+    c.a[0] = load_scales8<kFew>(ws, arow, st, nblk);
+    if constexpr (M == kGateUp) c.a[1] = load_scales8<kFew>(us, arow, st, nblk);
+#pragma unroll
+    for (int n = 0; n < NI; ++n) c.b[n] = load_scales8<kFew>(xs, brow[n], st, nblk);
+  };
+
+  f32x16_t acc[MI] = {};    // 32 rows
+  f32x4_t acc16[2] = {};    // 16 rows: two groups of 16 columns
+  auto multiply = [&](uint32_t s, uint32_t buf, const Scales &c) {
+    const ScaleStep st = scale_step(s, nblk);
+    const uint8_t *p = ring + buf * kBuf;
+    uint32_t sa[MI], sb[NI];
+#pragma unroll
+    for (int m = 0; m < MI; ++m) sa[m] = lane_scales(c.a[m], st, sel);
+#pragma unroll
+    for (int n = 0; n < NI; ++n) sb[n] = lane_scales(c.b[n], st, sel);
+    const uint32_t row = lane & (kRows - 1u), swz = (row >> 1) & 7u;
+    auto frag = [&](uint32_t first, uint32_t k) {
+      constexpr uint32_t kG = kRows == 32 ? 2u : 4u;
+      return *reinterpret_cast<const u32x4_t *>(p + (first + row) * 128u +
+                                                (((kG * k + group) ^ swz) * 16u));
+    };
+    if constexpr (kRows == 32) {
+      u32x4_t fa[MI][4], fb[4];
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+#pragma unroll
+        for (uint32_t m = 0; m < MI; ++m) fa[m][k] = frag(32u * m, k);
+        fb[k] = frag(kARows, k);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // read before the buffer is refilled
+      request(s + NB * NW, buf);
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        acc[m] = mfma<0>(fa[m][0], fb[0], acc[m], sa[m], sb[0]);
+        acc[m] = mfma<1>(fa[m][1], fb[1], acc[m], sa[m], sb[0]);
+        acc[m] = mfma<2>(fa[m][2], fb[2], acc[m], sa[m], sb[0]);
+        acc[m] = mfma<3>(fa[m][3], fb[3], acc[m], sa[m], sb[0]);
+      }
+    } else {
+      u32x4_t fa[2], fb[2][2];
+#pragma unroll
+      for (uint32_t k = 0; k < 2; ++k) {
+        fa[k] = frag(0, k);
+#pragma unroll
+        for (uint32_t n = 0; n < 2; ++n) fb[n][k] = frag(16u + 16u * n, k);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      request(s + NB * NW, buf);
+#pragma unroll
+      for (uint32_t n = 0; n < 2; ++n) {
+        acc16[n] = mfma16<0>(fa[0], fb[n][0], acc16[n], sa[0], sb[n]);
+        acc16[n] = mfma16<1>(fa[1], fb[n][1], acc16[n], sa[0], sb[n]);
+      }
+    }
+  };
+
+  // Everything that a step requests is requested in one go, so that the counter
+  // says which steps have landed: all but the NB - 1 younger ones.
+  constexpr int kStepLoads = kLoads + MI + NI;
+  if (nblk >= 8u) {
+    Scales c[NB];
+#pragma unroll
+    for (uint32_t i = 0; i < NB; ++i) {
+      load_scales(wave + i * NW, c[i], std::false_type());
+      request(wave + i * NW, i);
+    }
+    for (uint32_t s = wave; s < steps; s += NB * NW) {
+#pragma unroll
+      for (uint32_t i = 0; i < NB; ++i) {
+        const uint32_t at = s + i * NW;
+        if (at >= steps) break;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * kStepLoads) : "memory");
+        const Scales now = c[i];
+        load_scales(at + NB * NW, c[i], std::false_type());
+        multiply(at, i, now);
+      }
+    }
+  } else if (wave == 0u) { // one step, of fewer blocks than a load of scales has
+    Scales c;
+    load_scales(0, c, std::true_type());
+    request(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    multiply(0, 0, c);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // loads past the last step
+  __syncthreads();
+
+  // partial tiles: [wave][matrix or column group][quarter][lane]
+  f32x4_t *const part = reinterpret_cast<f32x4_t *>(lds);
+  constexpr uint32_t kQuarters = kRows == 32 ? 4u * MI : 2u;
+  if constexpr (kRows == 32) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        part[(wave * kQuarters + m * 4u + q) * 64u + lane] =
+            (f32x4_t){acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]};
+  } else {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) part[(wave * kQuarters + n) * 64u + lane] = acc16[n];
+  }
+  __syncthreads();
+  auto total = [&](uint32_t q) {
+    f32x4_t v = part[q * 64u + lane];
+#pragma unroll
+    for (uint32_t w = 1; w < NW; ++w) v += part[(w * kQuarters + q) * 64u + lane];
+    return v;
+  };
+  const bool whole = store_whole<T>(a.y, a.n_rows);
+  auto emit = [&](uint32_t j, uint32_t r, f32x4_t g, f32x4_t u) {
+    if (j >= t.count) return;
+    if (whole)
+      emit4<M, T, true>(a, slot_of(j), r, g, u);
+    else
+      emit4<M, T, false>(a, slot_of(j), r, g, u);
+  };
+  if constexpr (kPacked) {
+    if (wave == 0u) {
+      float h[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4_t g = total(q), u = total(4u * (MI - 1) + q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[4 * q + i] = swiglu(g[i], u[i]);
+      }
+      store_packed(a.y, a.ysc, (uint64_t)slot_of(r32) * (a.n_rows / 32u) + t.m, h, group,
+                   r32 < t.count);
+    }
+  } else if constexpr (kRows == 32) {
+    if (wave < 4u) {
+      const f32x4_t g = total(wave), u = M == kGateUp ? total(4u * (MI - 1) + wave) : g;
+      emit(r32, row0 + 8u * wave + 4u * group, g, u);
+    }
+  } else if (wave < 2u) {
+    const f32x4_t g = total(wave);
+    emit(16u * wave + (lane & 15u), row0 + 4u * group, g, g);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Tile kind: BM x BN outputs (gate/up: BM / 2 rows of each matrix, in turns of
+// 32), WM x WN waves, rows of at least sixteen blocks.  K goes in steps of 256
+// through NBUF LDS buffers filled by direct-to-LDS loads.  An LDS row is 128
+// bytes, the codes of one step (a whole line, so that eight lanes of a load are
+// one request to L2), with 16-byte piece c at place c ^ (row / 2 % 8): the
+// sixteen rows that a quarter of a fragment read touches (rows 0-3, 12-15, 20-23
+// and 24-27, or the others, of 32) then meet all the banks.  The scales of two
+// steps, 16 bytes a row, go through registers to LDS.
+//
+// A step is four parts of 64 columns; a part's fragments are read among the
+// products of the part before it.  One barrier a step, before its last part: by
+// then every wave has read its last fragments of the step, so its buffer is
+// refilled during the last part and the next step's first one, and has seen its
+// own loads of the next step land.
+// ---------------------------------------------------------------------------
+template <Mode M, class T, bool kPacked, int BM, int BN, int WM, int WN, int NBUF>
+__device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
+  constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
+  constexpr int kSRows = (BM + BN + 64 * NW - 1) / (64 * NW); // rows of scales per lane
+  constexpr uint32_t kBuf = (BM + BN) * 128u, kSBuf = kSRows * 64u * NW * 16u;
+  constexpr int kLoads = (BM + BN) / 8 / NW; // per wave and step; rows of A first
+  constexpr int kALoads = BM / 8 / NW;
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads per wave");
+  static_assert(NW % 2 == 0, "the rows of a lane's loads are alike mod 16");
+  static_assert(M != kGateUp || MI % 2 == 0, "gate and up rows in one wave");
+  constexpr uint32_t kRows = M == kGateUp ? BM / 2 : BM; // rows of y
+  uint8_t *const slds = lds + NBUF * kBuf;
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t wm = wave / WN, wn = wave % WN;
+  const uint32_t half = lane >> 5, r32 = lane & 31u;
+  const Tile t = tile_of<M, BN>(a);
+  if (!t.real) return;
+  const uint32_t row0 = t.m * kRows;
+  const uint32_t nblk = a.nblk, row_bytes = nblk * 16u;
+  const uint64_t wat = (uint64_t)t.expert * a.n_rows * nblk + (uint64_t)row0 * nblk;
+  const uint32_t rows = a.n_rows - row0 < kRows ? a.n_rows - row0 : kRows;
+  const __amdgpu_buffer_rsrc_t wc = rsrc(a.wc + wat * 16u, rows * row_bytes);
+  const __amdgpu_buffer_rsrc_t uc = M == kGateUp ? rsrc(a.uc + wat * 16u, rows * row_bytes) : wc;
+  const uint64_t xbase = M == kDense ? t.n0 : 0u;
+  const uint32_t xrows = M == kDense ? t.count : a.n_x;
+  const __amdgpu_buffer_rsrc_t xc = rsrc(a.xc + xbase * row_bytes, xrows * row_bytes);
   // row of X of column j of the tile, and the row of y that it gives
   auto slot_of = [&](uint32_t j) {
     return M == kDense ? t.n0 + j : plan_order(a)[t.first + (j < t.count ? j : 0u)];
   };
   auto xrow_of = [&](uint32_t j) { return M == kDense ? j : slot_of(j) / a.x_div; };
 
-  // this lane's part of each load: row 8 * (load * NW + wave) + lane / 8
-  const uint32_t l8 = lane >> 3, piece = (lane & 7u) ^ (l8 & 7u);
+  // this lane's part of each load of codes: row 8 * (load * NW + wave) + lane / 8
+  const uint32_t l8 = lane >> 3, piece = (lane & 7u) ^ ((4u * wave + (l8 >> 1)) & 7u);
   uint32_t off[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
@@ -424,123 +516,271 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
     }
   }
   const uint32_t steps = (nblk + 7u) / 8u;
-  auto fill = [&](uint32_t s, uint32_t buf) {
-    const bool in = 8u * s + piece < nblk; // false past the end of a last, partial step
+  // load i of step s into buffer buf; steps past the end: zeros
+  auto request = [&](uint32_t s, uint32_t buf, int i) {
+    const bool in = 8u * s + piece < nblk;
+    const uint32_t r8 = 8u * ((i < kALoads ? i : i - kALoads) * NW + wave);
+    const bool up = M == kGateUp && i < kALoads && ((r8 >> 5) & 1u);
+    uint8_t *to = lds + buf * kBuf + ((i < kALoads ? 0u : (uint32_t)BM) + r8) * 128u;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kALoads ? (up ? uc : wc) : xc, (lds_void_t *)to,
+                                             16, (int)(in ? off[i] + s * 128u : kFar), 0, 0, 0);
+  };
+
+  // scales: lane (64 * NW * i + thread) takes a row of A or of B (rows that there
+  // are not: the last one's, whose products are not stored)
+  const uint8_t *sbase[kSRows];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t load = i < kALoads ? i : i - kALoads;
-      const uint32_t r8 = 8u * (load * NW + wave);
-      const bool up = M == kGateUp && i < kALoads && ((r8 >> 5) & 1u);
-      uint8_t *to = lds + buf * kBuf + ((i < kALoads ? 0u : (uint32_t)BM) + r8) * 128u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kALoads ? (up ? uc : wc) : xc,
-                                               (lds_void_t *)to, 16, (int)(in ? off[i] : kFar),
-                                               (int)(s * 128u), 0, 0);
+  for (int i = 0; i < kSRows; ++i) {
+    const uint32_t r = 64u * NW * i + threadIdx.x;
+    if (r < (uint32_t)BM) {
+      uint32_t row = M == kGateUp ? (r >> 6) * 32u + (r & 31u) : r;
+      row = row < rows ? row : rows - 1u;
+      const bool up = M == kGateUp && ((r >> 5) & 1u);
+      sbase[i] = (up ? a.us : a.ws) + wat + (uint64_t)row * nblk;
+    } else { // (lanes past the rows of B repeat its last one)
+      const uint32_t j = r - BM;
+      sbase[i] = a.xs + (xbase + xrow_of(j < t.count ? j : t.count - 1u)) * nblk;
     }
-  };
-  // scales: the lane's row of each of the wave's 32-row operand tiles
-  uint32_t arow[MI], brow[NI];
-#pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    const uint32_t tile = wm * MI + m;
-    arow[m] = ((M == kGateUp ? tile >> 1 : tile) * 32u + r32) * nblk;
   }
+  // the scales of blocks 16 p .. 16 p + 15, read inside the row: at its end from
+  // further back, and shifted down by put_scales
+  u32x4_t sreg[kSRows];
+  const uint32_t last16 = nblk - 16u;
+  auto get_scales = [&](uint32_t p) {
+    const uint32_t at = 16u * p < last16 ? 16u * p : last16;
 #pragma unroll
-  for (int n = 0; n < NI; ++n) {
-    const uint32_t j = (wn * NI + n) * 32u + r32;
-    brow[n] = j < t.count ? xrow_of(j) * nblk : kFar;
-  }
-  struct Scales {
-    u32x2_t a[MI], b[NI];
-    ScaleStep st;
+    for (int i = 0; i < kSRows; ++i) __builtin_memcpy(&sreg[i], sbase[i] + at, 16);
   };
-  auto load_scales = [&](uint32_t s, Scales &p) {
-    p.st = scale_step(s, nblk);
+  auto put_scales = [&](uint32_t p) {
+    const uint32_t d = 16u * p < last16 ? 0u : 16u * p - last16; // bytes, 15 at most if p is real
+    const uint32_t bits = 8u * (d & 7u);
 #pragma unroll
-    for (int m = 0; m < MI; ++m)
-      p.a[m] = load_scales8(M == kGateUp && (m & 1) ? us : ws, arow[m], p.st, nblk);
-#pragma unroll
-    for (int n = 0; n < NI; ++n) p.b[n] = load_scales8(xs, brow[n], p.st, nblk);
+    for (int i = 0; i < kSRows; ++i) {
+      uint64_t lo = (uint64_t)sreg[i].y << 32 | sreg[i].x, hi = (uint64_t)sreg[i].w << 32 | sreg[i].z;
+      lo = d & 8u ? hi : lo;
+      hi = d & 8u ? 0u : hi;
+      lo = lo >> bits | (hi << 1) << (63u - bits);
+      hi >>= bits;
+      *reinterpret_cast<u32x4_t *>(slds + (p & 1u) * kSBuf + (64u * NW * i + threadIdx.x) * 16u) =
+          (u32x4_t){(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    }
   };
 
   f32x16_t acc[MI][NI] = {};
   const uint32_t sel = scale_selector(half);
-  uint32_t frag[4]; // byte offset of the lane's piece of K part kk in a 32-row tile
+  uint32_t frag[4]; // byte offset of the lane's piece of part kk in a 32-row tile
 #pragma unroll
-  for (uint32_t k = 0; k < 4; ++k) frag[k] = r32 * 128u + (((2u * k + half) ^ (r32 & 7u)) * 16u);
-  auto multiply = [&](const Scales &p, uint32_t buf) {
-    uint32_t sa[MI], sb[NI];
+  for (uint32_t k = 0; k < 4; ++k)
+    frag[k] = r32 * 128u + (((2u * k + half) ^ ((r32 >> 1) & 7u)) * 16u);
+  const uint32_t abase = wm * (MI * 4096u), bbase = BM * 128u + wn * (NI * 4096u);
+  struct Frags {
+    u32x4_t a[MI], b[NI];
+  };
+  auto read_frag = [&](Frags &f, int k, uint32_t buf, int i) {
+    const uint8_t *p = lds + buf * kBuf + frag[k];
+    if (i < MI)
+      f.a[i] = *reinterpret_cast<const u32x4_t *>(p + abase + i * 4096);
+    else
+      f.b[i - MI] = *reinterpret_cast<const u32x4_t *>(p + bbase + (i - MI) * 4096);
+  };
+  auto read_frags = [&](Frags &f, int k, uint32_t buf) {
 #pragma unroll
-    for (int m = 0; m < MI; ++m) sa[m] = lane_scales(p.a[m], p.st, sel);
+    for (int i = 0; i < MI + NI; ++i) read_frag(f, k, buf, i);
+  };
+  struct Scales { // of one step, a byte a part
+    uint32_t a[MI], b[NI];
+  };
+  auto read_scales = [&](Scales &c, uint32_t s) {
+    const uint8_t *q = slds + ((s >> 1) & 1u) * kSBuf + (s & 1u) * 8u + r32 * 16u;
 #pragma unroll
-    for (int n = 0; n < NI; ++n) sb[n] = lane_scales(p.b[n], p.st, sel);
-    const uint8_t *la = lds + buf * kBuf + wm * (MI * 4096u);
-    const uint8_t *lb = lds + buf * kBuf + BM * 128u + wn * (NI * 4096u);
-    auto part = [&](auto kk) {
-      constexpr int K = decltype(kk)::value;
-      u32x4_t fa[MI], fb[NI];
+    for (int m = 0; m < MI; ++m) {
+      const u32x2_t v = *reinterpret_cast<const u32x2_t *>(q + (wm * MI + m) * 512u);
+      c.a[m] = __builtin_amdgcn_perm(v.y, v.x, sel);
+    }
 #pragma unroll
-      for (int m = 0; m < MI; ++m)
-        fa[m] = *reinterpret_cast<const u32x4_t *>(la + m * 4096 + frag[K]);
+    for (int n = 0; n < NI; ++n) {
+      const u32x2_t v = *reinterpret_cast<const u32x2_t *>(q + BM * 16u + (wn * NI + n) * 512u);
+      c.b[n] = __builtin_amdgcn_perm(v.y, v.x, sel);
+    }
+  };
+  auto multiply = [&](const Frags &f, const Scales &c, auto kk) {
+    constexpr int K = decltype(kk)::value;
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
 #pragma unroll
       for (int n = 0; n < NI; ++n)
-        fb[n] = *reinterpret_cast<const u32x4_t *>(lb + n * 4096 + frag[K]);
+        acc[m][n] = mfma<K>(f.a[m], f.b[n], acc[m][n], c.a[m], c.b[n]);
+  };
+  constexpr std::integral_constant<int, 0> k0;
+  constexpr std::integral_constant<int, 1> k1;
+  constexpr std::integral_constant<int, 2> k2;
+  constexpr std::integral_constant<int, 3> k3;
+  auto after = [](uint32_t b) { return b + 1u == NBUF ? 0u : b + 1u; };
+  // What goes among a part's products: the next part's fragments f (part k of
+  // buffer from) and the requests [begin, end) of step s into buffer `to`.  The
+  // compiler keeps reads and requests in this order, both being accesses to LDS.
+  constexpr int kHalf = kLoads / 2, kReads = MI + NI;
+  auto loads = [&](Frags &f, int k, uint32_t from, uint32_t s, uint32_t to, int begin, int end) {
+    const int n = end - begin;
 #pragma unroll
-      for (int m = 0; m < MI; ++m)
+    for (int i = 0; i < kReads; ++i) {
+      read_frag(f, k, from, i);
 #pragma unroll
-        for (int n = 0; n < NI; ++n)
-          acc[m][n] = mfma<K>(fa[m], fb[n], acc[m][n], sa[m], sb[n]);
-    };
-    part(std::integral_constant<int, 0>());
-    part(std::integral_constant<int, 1>());
-    part(std::integral_constant<int, 2>());
-    part(std::integral_constant<int, 3>());
+      for (int r = begin + i * n / kReads; r < begin + (i + 1) * n / kReads; ++r)
+        request(s, to, r);
+    }
+  };
+  auto interleave = [&](auto requests) {
+    constexpr int kPer = (MI * NI + kReads - 1) / kReads, kN = decltype(requests)::value;
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);    // LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0); // MFMA
+      if (kN > 0) __builtin_amdgcn_sched_group_barrier(0x020, (kN + kReads - 1) / kReads, 0);
+    }
+  };
+  Frags f0, f1;
+  Scales c0, c1;
+  constexpr std::integral_constant<int, 0> kNone;
+  constexpr std::integral_constant<int, kHalf> kFirst;
+  constexpr std::integral_constant<int, kLoads - kHalf> kSecond;
+  // Step s is in buffer buf, step s + 1 in buffer then; before: buffer of step
+  // s - 1.  The scales of two steps come together, and early, as a load that is
+  // late holds up all the counted ones behind it: those of steps s + 3 and s + 4
+  // are requested in an odd step s, after the requests that its barrier waits for,
+  // and put into LDS in step s + 2.
+  auto step = [&](uint32_t s, auto odd, uint32_t before, uint32_t buf, uint32_t then,
+                  const Scales &c, Scales &next) {
+    constexpr bool kOdd = decltype(odd)::value;
+    __builtin_amdgcn_sched_barrier(0);
+    if (kOdd) put_scales((s >> 1) + 1u); // read after the barrier
+    loads(f1, 1, buf, s + NBUF - 1u, before, kHalf, kLoads);
+    multiply(f0, c, k0);
+    interleave(kSecond);
+    __builtin_amdgcn_sched_barrier(0);
+    if (kOdd) get_scales((s >> 1) + 2u); // behind the requests above
+    read_frags(f0, 2, buf);
+    multiply(f1, c, k1);
+    interleave(kNone);
+    __builtin_amdgcn_sched_barrier(0);
+    read_frags(f1, 3, buf);
+    multiply(f0, c, k2);
+    interleave(kNone);
+    __builtin_amdgcn_sched_barrier(0);
+    // step s + 1 has landed: of the younger loads, NBUF - 2 steps' and, in an odd step
+    // or with a third buffer, the scales', may be on their way
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
+                     (NBUF - 2) * kLoads + (kOdd || NBUF > 2 ? kSRows : 0))
+                 : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    loads(f0, 0, then, s + NBUF, buf, 0, kHalf);
+    multiply(f1, c, k3);
+    interleave(kFirst);
+    read_scales(next, s + 1u);
   };
 
-  Scales p0, p1;
-  load_scales(0, p0);
-  fill(0, 0);
+  get_scales(0);
+#pragma unroll
+  for (uint32_t s = 0; s < NBUF; ++s)
+#pragma unroll
+    for (int i = 0; i < (s + 1u < NBUF ? kLoads : kHalf); ++i) request(s, s, i);
+  put_scales(0);
+  get_scales(1);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 2) * kLoads + kHalf +
+                                                                  kSRows)
+               : "memory");
+  read_frags(f0, 0, 0);
+  read_scales(c0, 0);
+  // Groups of two steps, zeros past the last one.  No branch inside: the compiler
+  // moves products over one, and then past the barriers, which leaves the loads
+  // nothing to hide behind.
+  uint32_t b0 = 0, before = NBUF - 1u;
   for (uint32_t s = 0; s < steps; s += 2u) {
-    // step s has landed everywhere, and nobody reads the other buffer any more
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 1u < steps) {
-      load_scales(s + 1u, p1);
-      fill(s + 1u, 1);
-    }
-    multiply(p0, 0);
-    if (s + 1u >= steps) break;
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 2u < steps) {
-      load_scales(s + 2u, p0);
-      fill(s + 2u, 0);
-    }
-    multiply(p1, 1);
+    const uint32_t b1 = after(b0), b2 = after(b1);
+    step(s, std::false_type(), before, b0, b1, c0, c1);
+    step(s + 1u, std::true_type(), b0, b1, b2, c1, c0);
+    before = b1;
+    b0 = b2;
   }
 
+  // Loads past the last step have landed and every wave is done with LDS: it holds
+  // the waves' results next.  What follows is not computed ahead of the loop, where
+  // registers are few.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  uint32_t tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const uint32_t l = tid & 63u, col32 = tid & 31u, half4 = (tid >> 5 & 1u) * 4u;
+  constexpr int kStep = M == kGateUp ? 2 : 1, kBlocks = MI / kStep; // 32-row blocks of a wave
+  const uint32_t wrow0 = row0 + wm * (kBlocks * 32u);               // the wave's first row of y
+  if constexpr (kPacked) {
 #pragma unroll
-  for (int n = 0; n < NI; ++n) {
-    const uint32_t j = (wn * NI + n) * 32u + r32;
-    const bool real = j < t.count;
-    const uint32_t out = slot_of(j);
-    constexpr int kStep = M == kGateUp ? 2 : 1;
+    for (int n = 0; n < NI; ++n) {
+      const uint32_t j = (wn * NI + n) * 32u + col32;
+      const uint32_t out = slot_of(j);
 #pragma unroll
-    for (int m = 0; m < MI; m += kStep) {
-      const uint32_t block = (wm * MI + m) / kStep; // 32-row block of the tile
-      const f32x16_t &g = acc[m][n], &u = acc[M == kGateUp ? m + 1 : m][n];
-      if constexpr (kPacked) {
+      for (int m = 0; m < MI; m += kStep) {
         float h[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) h[i] = swiglu(g[i], u[i]);
-        const uint32_t fb = row0 / 32u + block;
-        store_packed(a.y, a.ysc, (uint64_t)out * (a.n_rows / 32u) + fb, h, half,
-                     real && fb < a.n_rows / 32u);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (real)
-            emit4<M, T>(a, out, row0 + block * 32u + 8u * q + 4u * half,
-                        (f32x4_t){g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]},
-                        (f32x4_t){u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]});
+        for (int i = 0; i < 16; ++i) h[i] = swiglu(acc[m][n][i], acc[m + kStep - 1][n][i]);
+        const uint32_t fb = wrow0 / 32u + m / kStep;
+        store_packed(a.y, a.ysc, (uint64_t)out * (a.n_rows / 32u) + fb, h, half4 / 4u,
+                     j < t.count && fb < a.n_rows / 32u);
       }
+    }
+  } else {
+    // A column of the wave's block after another in LDS (with 16 bytes between, so
+    // that the columns of a write meet all the banks), and from there in whole
+    // rows of 16-byte pieces: a store instruction then writes 256 to 512
+    // consecutive bytes of a column of y in place of 32 bytes of 32 columns.
+    constexpr uint32_t kColBytes = kBlocks * 32u * T::kBytes, kPitch = kColBytes + 16u;
+    constexpr uint32_t kLanes = kColBytes / 16u, kCols = 64u / kLanes; // lanes of a column
+    constexpr uint32_t kPer = 16u / T::kBytes;                         // rows of a piece
+    static_assert(NW * 32u * kPitch <= NBUF * kBuf + 2u * kSBuf, "the columns fit LDS");
+    uint8_t *const mine = lds + wave * (32u * kPitch);
+    const uint32_t c0_ = l / kLanes, piece_row = (l % kLanes) * kPer;
+    const bool whole = a.n_rows % kPer == 0u && ((uintptr_t)a.y & 15u) == 0u;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const uint32_t j0 = (wn * NI + n) * 32u;
+#pragma unroll
+      for (int m = 0; m < MI; m += kStep)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4_t v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] = M == kGateUp ? swiglu(acc[m][n][4 * q + i], acc[m + kStep - 1][n][4 * q + i])
+                                : acc[m][n][4 * q + i];
+          uint8_t *p = mine + col32 * kPitch + ((m / kStep) * 32u + 8u * q + half4) * T::kBytes;
+          if constexpr (T::kBytes == 4)
+            *reinterpret_cast<f32x4_t *>(p) = v;
+          else
+            *reinterpret_cast<u32x2_t *>(p) =
+                (u32x2_t){pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the wave's own writes
+#pragma unroll 4
+      for (uint32_t c = 0; c < 32u; c += kCols) {
+        const uint32_t j = j0 + c + c0_, r = wrow0 + piece_row;
+        const u32x4_t v =
+            *reinterpret_cast<const u32x4_t *>(mine + (c + c0_) * kPitch + (l % kLanes) * 16u);
+        if (j < t.count && r < a.n_rows) {
+          uint8_t *to = a.y + ((uint64_t)slot_of(j) * a.n_rows + r) * T::kBytes;
+          if (whole) {
+            *reinterpret_cast<u32x4_t *>(to) = v;
+          } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i)
+              if (r + i < a.n_rows) {
+                if constexpr (T::kBytes == 4)
+                  reinterpret_cast<uint32_t *>(to)[i] = v[i];
+                else
+                  reinterpret_cast<uint16_t *>(to)[i] = (uint16_t)(v[i / 2u] >> (16u * (i % 2u)));
+              }
+          }
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // read before the next columns come
     }
   }
 }
@@ -561,65 +801,73 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   const Args a{wc, ws, uc, us, xc, xs, plan, y, ysc, n_rows, nblk, 0u, n_x, x_div, n_experts,     \
                row_tiles}
 
-// Skinny kernels: NI column groups of 32, NW waves.
-#define AXH_MX_SKINNY(TN, T, NI, NW)                                                              \
+// K-split kernels: kRows rows, NW waves, NB buffers of each.
+#define AXH_MX_KSPLIT(NAME, TN, T, ROWS, NW, NB)                                                  \
   extern "C" __global__ void __launch_bounds__(64 * NW)                                           \
-      axh_mxfp4_matmul_s##NI##_##TN(AXH_MX_DENSE_ARGS) {                                          \
-    extern __shared__ f32x4_t part[];                                                             \
+      axh_mxfp4_matmul_##NAME##_##TN(AXH_MX_DENSE_ARGS) {                                         \
+    extern __shared__ __align__(16) uint8_t ring[];                                               \
     AXH_MX_DENSE_UNPACK;                                                                          \
-    skinny_body<kDense, T, false, NI, NW>(a, part);                                               \
+    ksplit_body<kDense, T, false, ROWS, NW, NB>(a, ring);                                         \
   }                                                                                               \
   extern "C" __global__ void __launch_bounds__(64 * NW)                                           \
-      axh_mxfp4_expert_matmul_s##NI##_##TN(AXH_MX_EXPERT_ARGS) {                                  \
-    extern __shared__ f32x4_t part[];                                                             \
+      axh_mxfp4_expert_matmul_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {                                 \
+    extern __shared__ __align__(16) uint8_t ring[];                                               \
     AXH_MX_EXPERT_UNPACK;                                                                         \
-    skinny_body<kGrouped, T, false, NI, NW>(a, part);                                             \
+    ksplit_body<kGrouped, T, false, ROWS, NW, NB>(a, ring);                                       \
   }
-#define AXH_MX_SKINNY_GU(TN, T, PACKED, NI, NW)                                                   \
+#define AXH_MX_KSPLIT_GU(NAME, TN, T, PACKED, NW, NB)                                             \
   extern "C" __global__ void __launch_bounds__(64 * NW)                                           \
-      axh_mxfp4_expert_gate_up_s##NI##_##TN(AXH_MX_EXPERT_ARGS) {                                 \
-    extern __shared__ f32x4_t part[];                                                             \
+      axh_mxfp4_expert_gate_up_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {                                \
+    extern __shared__ __align__(16) uint8_t ring[];                                               \
     AXH_MX_EXPERT_UNPACK;                                                                         \
-    skinny_body<kGateUp, T, PACKED, NI, NW>(a, part);                                             \
+    ksplit_body<kGateUp, T, PACKED, 32, NW, NB>(a, ring);                                         \
   }
-#define AXH_MX_SKINNY_N(NI, NW, NWG)              \
-  AXH_MX_SKINNY(f32, TF32, NI, NW)                \
-  AXH_MX_SKINNY(f16, TF16, NI, NW)                \
-  AXH_MX_SKINNY(bf16, TBF16, NI, NW)              \
-  AXH_MX_SKINNY_GU(f32, TF32, false, NI, NWG)     \
-  AXH_MX_SKINNY_GU(f16, TF16, false, NI, NWG)     \
-  AXH_MX_SKINNY_GU(bf16, TBF16, false, NI, NWG)   \
-  AXH_MX_SKINNY_GU(mxfp4, TF32, true, NI, NWG)
-AXH_MX_SKINNY_N(1, 8, 8)
-AXH_MX_SKINNY_N(2, 8, 4)
+#define AXH_MX_KSPLIT_N(NAME, ROWS, NW, NB)        \
+  AXH_MX_KSPLIT(NAME, f32, TF32, ROWS, NW, NB)     \
+  AXH_MX_KSPLIT(NAME, f16, TF16, ROWS, NW, NB)     \
+  AXH_MX_KSPLIT(NAME, bf16, TBF16, ROWS, NW, NB)
+#define AXH_MX_KSPLIT_GU_N(NAME, NW, NB)                 \
+  AXH_MX_KSPLIT_GU(NAME, f32, TF32, false, NW, NB)       \
+  AXH_MX_KSPLIT_GU(NAME, f16, TF16, false, NW, NB)       \
+  AXH_MX_KSPLIT_GU(NAME, bf16, TBF16, false, NW, NB)     \
+  AXH_MX_KSPLIT_GU(NAME, mxfp4, TF32, true, NW, NB)
+AXH_MX_KSPLIT_N(k16, 16, 8, 3)
+AXH_MX_KSPLIT_N(k32, 32, 8, 2)
+AXH_MX_KSPLIT_GU_N(k32, 4, 3)
 
 // Tile kernels.
-#define AXH_MX_TILE(NAME, TN, T, BM, BN, WM, WN)                                                  \
+#define AXH_MX_TILE(NAME, TN, T, BM, BN, WM, WN, NBUF, WPE)                                             \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN)                                      \
+      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                                              \
       axh_mxfp4_matmul_##NAME##_##TN(AXH_MX_DENSE_ARGS) {                                         \
     extern __shared__ __align__(16) uint8_t tile[];                                                       \
     AXH_MX_DENSE_UNPACK;                                                                          \
-    tile_body<kDense, T, false, BM, BN, WM, WN>(a, tile);                                         \
+    tile_body<kDense, T, false, BM, BN, WM, WN, NBUF>(a, tile);                                         \
   }                                                                                               \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN)                                      \
+      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                                              \
       axh_mxfp4_expert_matmul_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {                                 \
     extern __shared__ __align__(16) uint8_t tile[];                                                       \
     AXH_MX_EXPERT_UNPACK;                                                                         \
-    tile_body<kGrouped, T, false, BM, BN, WM, WN>(a, tile);                                       \
+    tile_body<kGrouped, T, false, BM, BN, WM, WN, NBUF>(a, tile);                                       \
   }
-#define AXH_MX_TILE_GU(NAME, TN, T, PACKED, BM, BN, WM, WN)                                       \
+#define AXH_MX_TILE_GU(NAME, TN, T, PACKED, BM, BN, WM, WN, NBUF, WPE)                                  \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN)                                      \
+      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                                              \
       axh_mxfp4_expert_gate_up_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {                                \
     extern __shared__ __align__(16) uint8_t tile[];                                                       \
     AXH_MX_EXPERT_UNPACK;                                                                         \
-    tile_body<kGateUp, T, PACKED, BM, BN, WM, WN>(a, tile);                                       \
+    tile_body<kGateUp, T, PACKED, BM, BN, WM, WN, NBUF>(a, tile);                                       \
   }
-#define AXH_MX_TILE_N(NAME, BM, BN, WM, WN)                        \
-  AXH_MX_TILE(NAME, f32, TF32, BM, BN, WM, WN)                     \
-  AXH_MX_TILE(NAME, f16, TF16, BM, BN, WM, WN)                     \
-  AXH_MX_TILE(NAME, bf16, TBF16, BM, BN, WM, WN)                   \
-  AXH_MX_TILE_GU(NAME, f32, TF32, false, BM, BN, WM, WN)           \
-  AXH_MX_TILE_GU(NAME, f16, TF16, false, BM, BN, WM, WN)           \
-  AXH_MX_TILE_GU(NAME, bf16, TBF16, false, BM, BN, WM, WN)         \
-  AXH_MX_TILE_GU(NAME, mxfp4, TF32, true, BM, BN, WM, WN)
-AXH_MX_TILE_N(t128x128, 128, 128, 2, 2)
+#define AXH_MX_TILE_N(NAME, BM, BN, WM, WN, NBUF, WPE)                   \
+  AXH_MX_TILE(NAME, f32, TF32, BM, BN, WM, WN, NBUF, WPE)                \
+  AXH_MX_TILE(NAME, f16, TF16, BM, BN, WM, WN, NBUF, WPE)                \
+  AXH_MX_TILE(NAME, bf16, TBF16, BM, BN, WM, WN, NBUF, WPE)              \
+  AXH_MX_TILE_GU(NAME, f32, TF32, false, BM, BN, WM, WN, NBUF, WPE)      \
+  AXH_MX_TILE_GU(NAME, f16, TF16, false, BM, BN, WM, WN, NBUF, WPE)      \
+  AXH_MX_TILE_GU(NAME, bf16, TBF16, false, BM, BN, WM, WN, NBUF, WPE)    \
+  AXH_MX_TILE_GU(NAME, mxfp4, TF32, true, BM, BN, WM, WN, NBUF, WPE)
+AXH_MX_TILE_N(t64x64, 64, 64, 1, 2, 3, 1)
+AXH_MX_TILE_N(t64x128, 64, 128, 1, 4, 3, 2)
+AXH_MX_TILE_N(t128x128, 128, 128, 2, 2, 2, 2)
+AXH_MX_TILE_N(t256x256, 256, 256, 2, 4, 2, 2)

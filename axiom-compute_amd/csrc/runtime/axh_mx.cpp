@@ -99,30 +99,41 @@ MatvecPlan plan_matvec(uint32_t n_rows, uint32_t nblk, uint32_t picks, uint32_t 
 // ---- matmul kernels -----------------------------------------------------------
 struct MatmulKind {
   const char *name;
-  uint32_t rows, cols;         // a workgroup's outputs (gate/up: rows / 2 of each matrix)
-  uint32_t threads, threads_gu; // gate/up: rows of both matrices
+  uint32_t rows, cols;   // a workgroup's outputs
+  uint32_t rows_gu;      // rows of each matrix (gate/up), 0 where there is none
+  uint32_t threads, threads_gu;
   uint32_t lds, lds_gu;
-  bool skinny;
 };
-constexpr MatmulKind kKinds[] = {
-    {"s1", 32, 32, 512, 512, 32768, 65536, true},
-    {"s2", 32, 64, 512, 256, 65536, 65536, true},
-    {"t128x128", 128, 128, 256, 256, 65536, 65536, false},
+// From the largest tile to the smallest; keep in sync with mx_matmul.hip.
+constexpr MatmulKind kTiles[] = {
+    {"t256x256", 256, 256, 128, 512, 512, 147456, 147456},
+    {"t128x128", 128, 128, 64, 256, 256, 73728, 73728},
+    {"t64x128", 64, 128, 32, 256, 256, 81920, 81920},
+    {"t64x64", 64, 64, 32, 128, 128, 53248, 53248},
 };
+constexpr MatmulKind kSplit32 = {"k32", 32, 32, 32, 512, 256, 131072, 147456};
+constexpr MatmulKind kSplit16 = {"k16", 16, 32, 0, 512, 0, 147456, 0};
+constexpr uint32_t kTileMinBlocks = 16; // the tiles read 16 scales of a row at once
+constexpr uint32_t kFullGrid = 200, kLongBlocks = 256;
 
 const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
-  (void)n_rows;
-  (void)nblk;
-  if (batch <= 32u) return kKinds[0];
-  if (batch <= 64u) return kKinds[1];
-  return kKinds[2];
+  auto grid = [&](const MatmulKind &k) {
+    return (uint64_t)div_up(n_rows, k.rows) * div_up(batch, k.cols);
+  };
+  if (nblk < kTileMinBlocks) return kSplit32;
+  for (const MatmulKind &k : kTiles)
+    if (grid(k) >= kFullGrid && (batch > k.cols / 2u || k.cols == 64u)) return k;
+  if (grid(kSplit32) <= 256u || nblk >= kLongBlocks)
+    return grid(kSplit16) <= 256u && nblk >= kLongBlocks ? kSplit16 : kSplit32;
+  return kTiles[3];
 }
 
-const MatmulKind &expert_kind(uint64_t slots, uint32_t n_experts) {
+const MatmulKind &expert_kind(uint64_t slots, uint32_t n_experts, uint32_t nblk) {
   const uint64_t mean = slots / n_experts;
-  if (mean <= 24u) return kKinds[0];
-  if (mean <= 64u) return kKinds[1];
-  return kKinds[2];
+  if (nblk < kTileMinBlocks || mean <= 16u) return kSplit32;
+  if (mean >= 192u) return kTiles[0];
+  if (mean >= 96u) return kTiles[1];
+  return kTiles[3];
 }
 
 // Shared checks of the expert products for prompts.
@@ -143,11 +154,11 @@ axh_status expert_launch(axh_context *ctx, const char *op, const char *type, boo
                          uint32_t x_div, uint64_t slots, uint32_t n_experts, void *stream) {
   if ((uint64_t)n_x * (cols / 2u) >= kMaxBuffer)
     return bad("the activations' codes must be below 2 GiB");
-  const MatmulKind &k = expert_kind(slots, n_experts);
+  const MatmulKind &k = expert_kind(slots, n_experts, cols / 32u);
   // the experts' last tiles are partial: at most so many tiles in all
   const uint64_t active = std::min<uint64_t>(n_experts, slots);
   const uint64_t tiles = active + (slots - active) / k.cols;
-  const uint32_t rows = gate_up && !k.skinny ? k.rows / 2u : k.rows;
+  const uint32_t rows = gate_up ? k.rows_gu : k.rows;
   const uint32_t row_tiles = div_up(n_rows, rows);
   const uint32_t words[] = {n_rows, cols / 32u, n_x, x_div, n_experts, row_tiles};
   return launch(ctx, kMatmul, std::string("axh_mxfp4_") + op + "_" + k.name + "_" + type,
