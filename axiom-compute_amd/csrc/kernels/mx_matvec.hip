@@ -4,9 +4,9 @@
 //
 // The axis that is summed over is cut into units of LPR blocks of 32 columns
 // (LPR = 64, or 32 or 16 where a row has no more blocks than that): a lane has
-// one block of a unit, its 32 activations stay in VGPRs for every row that the
-// wave takes, so neither LDS traffic nor a cross-lane step stands between the
-// weight loads and the multiplications.  A load instruction of a wave reads 64
+// one block of a unit, its 32 activations, once staged, stay in VGPRs for every
+// row that the wave takes, so neither LDS traffic nor a cross-lane step stands
+// between the weight loads and the multiplications.  A load instruction of a wave reads 64
 // consecutive blocks (1 KiB of codes) of 64 / LPR rows.  The waves of a group
 // have a unit each and the same rows; a group's partial sums meet in LDS, in
 // the units' order.
@@ -16,19 +16,17 @@ using namespace axh;
 
 namespace {
 
+typedef __attribute__((address_space(3))) void lds_void_t;
+
 enum Mode { kDense, kGateUp, kDown };
 
 // Offset of lanes past a row's last block.  The row's offset is added to it: the
 // host keeps the rows of a group below 1 GiB, so the sum is past every buffer's
 // end and below 2^32, and such loads return zeros.
 constexpr uint32_t kFar = 0x80000000u;
-constexpr int kR = 8; // load instructions (rows times 64 / LPR) per batch
-
-// The codes and scales of one batch.
-struct Batch {
-  u32x4_t c[kR];
-  uint32_t s[kR];
-};
+// Load instructions of a batch, of 64 / LPR rows each: fewer where a group's waves
+// share out the choices of a token, so that there are more groups.
+template <Mode M> constexpr int kLoadsOf = M == kDown ? 4 : 8;
 
 __device__ __forceinline__ f32x2_t swap32_f(float a, float b) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a),
@@ -76,7 +74,7 @@ struct Shape {
   uint32_t n_rows;  // output rows (gate/up: of each matrix)
   uint32_t nblk;    // blocks of a row
   uint32_t uw;      // waves of a group
-  uint32_t batches; // batches of a group
+  uint32_t batches; // batches of a group, even
   uint32_t top_k, n_experts;
 };
 
@@ -94,10 +92,15 @@ template <Mode M, int LPR>
 __device__ __forceinline__ void
 matvec_body(const uint8_t *wc, const uint8_t *ws, const uint8_t *wc2, const uint8_t *ws2,
             const float *x, const int32_t *experts, const float *weights, float *y, Shape a,
-            float *lds) {
+            uint8_t *lds_bytes) {
+  constexpr int kR = kLoadsOf<M>;
   constexpr uint32_t kPer = 64u / LPR;                       // rows of a load instruction
   constexpr uint32_t kMats = M == kGateUp ? 2u : 1u;
   constexpr uint32_t kBatchRows = kR * kPer / kMats;         // rows of a batch, per matrix
+  struct Batch { // codes and scales
+    u32x4_t c[kR];
+    uint32_t s[kR];
+  };
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t group = wave / a.uw, u0 = wave - group * a.uw;
@@ -111,6 +114,9 @@ matvec_body(const uint8_t *wc, const uint8_t *ws, const uint8_t *wc2, const uint
   const uint32_t count = left < group_rows ? left : group_rows;
   const uint64_t matrix = (uint64_t)a.n_rows * a.nblk; // blocks of one expert
   const uint32_t item = blockIdx.y;                    // gate/up: slot; down: token
+  // LDS: a unit's activations per wave, then the partial sums
+  uint8_t *const stage = lds_bytes + wave * (LPR * 128u);
+  float *const lds = reinterpret_cast<float *>(lds_bytes + (blockDim.x >> 6) * (LPR * 128u));
   float *mine = lds + group * (group_rows * kMats * a.uw);
 
   uint32_t only = 0; // gate/up: the slot's expert
@@ -170,26 +176,25 @@ matvec_body(const uint8_t *wc, const uint8_t *ws, const uint8_t *wc2, const uint
             mine[r * a.uw + u0] += sum;
         }
       };
+      // Sums over the lanes of a row: exchanges of half the values between half
+      // the lanes, then DPP steps inside 16 lanes.
       if constexpr (LPR == 64) {
-        float h[4], q[2];
+        float h[kR / 2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x2_t p = swap32_f(v[i], v[i + 4]);
+        for (int i = 0; i < kR / 2; ++i) {
+          const f32x2_t p = swap32_f(v[i], v[i + kR / 2]);
           h[i] = p.x + p.y;
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f32x2_t p = swap16_f(h[i], h[i + 2]);
-          q[i] = p.x + p.y;
+        for (uint32_t i = 0; i < kR / 4; ++i) {
+          const f32x2_t p = swap16_f(h[i], h[i + kR / 4]);
+          put(i + (kR / 4) * ((lane >> 4) & 1u) + (kR / 2) * (lane >> 5), row_sum16(p.x + p.y));
         }
-#pragma unroll
-        for (uint32_t i = 0; i < 2; ++i)
-          put(i + 2u * ((lane >> 4) & 1u) + 4u * (lane >> 5), row_sum16(q[i]));
       } else if constexpr (LPR == 32) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const f32x2_t p = swap16_f(v[i], v[i + 4]);
-          put(i + 4u * ((lane >> 4) & 1u), row_sum16(p.x + p.y));
+        for (uint32_t i = 0; i < kR / 2; ++i) {
+          const f32x2_t p = swap16_f(v[i], v[i + kR / 2]);
+          put(i + (kR / 2) * ((lane >> 4) & 1u), row_sum16(p.x + p.y));
         }
       } else {
 #pragma unroll
@@ -197,26 +202,39 @@ matvec_body(const uint8_t *wc, const uint8_t *ws, const uint8_t *wc2, const uint
       }
     };
 
+    // The unit's activations, 128 bytes a lane, come through LDS in whole lines
+    // (loaded by the lanes themselves, an instruction would touch 64 lines for 16
+    // bytes of each); 16-byte piece p of block b at place p ^ (b / 2 % 8), so that
+    // the reads of 64 blocks' pieces meet all the banks.
+    const __amdgpu_buffer_rsrc_t xb = rsrc(xu, a.nblk * 128u);
+#pragma unroll
+    for (uint32_t i = 0; i < LPR / 8; ++i) {
+      const uint32_t b = 8u * i + (lane >> 3), p = (lane & 7u) ^ ((b >> 1) & 7u);
+      const uint32_t at = chunk * 64u + b;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (lds_void_t *)(stage + i * 1024u), 16,
+                                               (int)(at < a.nblk ? at * 128u + p * 16u : kFar), 0,
+                                               0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     Batch t0, t1;
     load(0, t0);
-    const __amdgpu_buffer_rsrc_t xb = rsrc(xu, a.nblk * 128u);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kR) : "memory"); // all but the batch
     f32x4_t xr[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const u32x4_t w =
-          __builtin_amdgcn_raw_buffer_load_b128(xb, in ? (int)(blk * 128u + 16u * i) : (int)kFar,
-                                                0, 0);
-      xr[i] = __builtin_bit_cast(f32x4_t, w);
-    }
-    // batches past the group's last row read zeros
+    for (uint32_t i = 0; i < 8; ++i)
+      xr[i] = *reinterpret_cast<const f32x4_t *>(stage + bl * 128u + ((i ^ ((bl >> 1) & 7u)) * 16u));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // read before another unit's come
+    // An even number of batches (those past the last row read zeros), so that the
+    // loop has one way through and the compiler's waits count the loads on it.
     uint32_t b = 0;
-    for (; b + 1u < a.batches; b += 2u) {
+    do {
       load(b + 1u, t1);
       finish(b, t0, xr);
       load(b + 2u, t0);
       finish(b + 1u, t1, xr);
-    }
-    if (b < a.batches) finish(b, t0, xr);
+      b += 2u;
+    } while (b < a.batches);
   }
   __syncthreads();
   for (uint32_t r = threadIdx.x; r < groups * group_rows; r += blockDim.x) {
@@ -242,7 +260,7 @@ matvec_body(const uint8_t *wc, const uint8_t *ws, const uint8_t *wc2, const uint
   extern "C" __global__ void __launch_bounds__(512) axh_mxfp4_matvec_l##LPR(                     \
       const uint8_t *wc, const uint8_t *ws, const float *x, float *y, uint32_t n_rows,            \
       uint32_t nblk, uint32_t uw, uint32_t batches) {                                             \
-    extern __shared__ float lds[];                                                                \
+    extern __shared__ __align__(16) uint8_t lds[];                                                \
     matvec_body<kDense, LPR>(wc, ws, nullptr, nullptr, x, nullptr, nullptr, y,                    \
                              Shape{n_rows, nblk, uw, batches, 1, 1}, lds);                        \
   }                                                                                               \
@@ -250,7 +268,7 @@ matvec_body(const uint8_t *wc, const uint8_t *ws, const uint8_t *wc2, const uint
       const uint8_t *gc, const uint8_t *gs, const uint8_t *uc, const uint8_t *us, const float *x, \
       const int32_t *experts, float *h, uint32_t n_rows, uint32_t nblk, uint32_t uw,              \
       uint32_t batches, uint32_t top_k, uint32_t n_experts) {                                     \
-    extern __shared__ float lds[];                                                                \
+    extern __shared__ __align__(16) uint8_t lds[];                                                \
     matvec_body<kGateUp, LPR>(gc, gs, uc, us, x, experts, nullptr, h,                             \
                               Shape{n_rows, nblk, uw, batches, top_k, n_experts}, lds);           \
   }                                                                                               \
@@ -258,7 +276,7 @@ matvec_body(const uint8_t *wc, const uint8_t *ws, const uint8_t *wc2, const uint
       const uint8_t *wc, const uint8_t *ws, const float *h, const int32_t *experts,               \
       const float *weights, float *y, uint32_t n_rows, uint32_t nblk, uint32_t uw,                \
       uint32_t batches, uint32_t top_k, uint32_t n_experts) {                                     \
-    extern __shared__ float lds[];                                                                \
+    extern __shared__ __align__(16) uint8_t lds[];                                                \
     matvec_body<kDown, LPR>(wc, ws, nullptr, nullptr, h, experts, weights, y,                     \
                             Shape{n_rows, nblk, uw, batches, top_k, n_experts}, lds);             \
   }

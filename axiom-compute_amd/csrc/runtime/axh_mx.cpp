@@ -78,21 +78,29 @@ struct MatvecPlan {
 };
 
 // `picks`: units of the summed axis beside the row's own (down: choices);
-// `mats`: matrices that a batch covers; `items`: workgroups along y.
-MatvecPlan plan_matvec(uint32_t n_rows, uint32_t nblk, uint32_t picks, uint32_t mats,
-                       uint32_t items) {
+// `loads`: load instructions of a batch, shared by `mats` matrices; `items`:
+// workgroups along y.
+//   A workgroup has 4 waves (or a wave for each unit, up to 8) where that makes
+// 256 workgroups of two batches, else one group.  Four batches where they make
+// one round of workgroups: 14336 x 4096 8.86 us against 9.07 with two, 8192 x
+// 8192 9.94 / 10.29, but 128256 x 4096 49.3 / 46.7 (fewer, and 4096 x 14336
+// 11.98 / 9.44).
+MatvecPlan plan_matvec(uint32_t n_rows, uint32_t nblk, uint32_t picks, uint32_t loads,
+                       uint32_t mats, uint32_t items) {
   MatvecPlan p{};
   p.lanes = nblk <= 16u ? 16u : nblk <= 32u ? 32u : 64u;
   const uint64_t units = (uint64_t)picks * (p.lanes == 64u ? div_up(nblk, 64u) : 1u);
   p.uw = (uint32_t)std::min<uint64_t>(units, 8u);
-  const uint32_t batch_rows = 8u * (64u / p.lanes) / mats;
-  const uint32_t batches = div_up(n_rows, batch_rows);
-  p.groups = std::max(1u, std::min(4u / p.uw, batches));
-  const uint64_t all = (uint64_t)batches * items;
-  p.batches = (uint32_t)std::min<uint64_t>(8u, std::max<uint64_t>(1u, all / (p.groups * 1024u)));
+  const uint32_t batch_rows = loads * (64u / p.lanes) / mats;
+  const uint64_t batches = (uint64_t)div_up(n_rows, batch_rows) * items;
+  p.groups = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>(4u / p.uw, batches / 512u));
+  auto grid = [&](uint32_t b) {
+    return (uint64_t)div_up(n_rows, (uint64_t)p.groups * b * batch_rows) * items;
+  };
+  p.batches = grid(4) >= 200u && grid(4) <= 512u ? 4u : 2u;
   p.group_rows = p.batches * batch_rows;
   p.wgs = div_up(n_rows, (uint64_t)p.groups * p.group_rows);
-  p.lds = p.groups * p.group_rows * mats * p.uw * 4u;
+  p.lds = p.groups * p.uw * (p.lanes * 128u + p.group_rows * mats * 4u);
   return p;
 }
 
@@ -270,7 +278,7 @@ axh_status axh_mxfp4_matvec(axh_context *ctx, const void *codes, const void *sca
   if (!aligned(codes, 16) || !aligned(x, 16) || !aligned(y, 4))
     return bad("codes and x must be 16-byte and y 4-byte aligned");
   const uint32_t nblk = cols / 32u;
-  const MatvecPlan p = plan_matvec(n_rows, nblk, 1, 1, 1);
+  const MatvecPlan p = plan_matvec(n_rows, nblk, 1, 8, 1, 1);
   const uint32_t words[] = {n_rows, nblk, p.uw, p.batches};
   void *bufs[] = {mut(codes), mut(scales), mut(x), y};
   return launch(ctx, kMatvec, "axh_mxfp4_matvec_l" + std::to_string(p.lanes), p.wgs, 1,
@@ -367,7 +375,7 @@ axh_status axh_mxfp4_expert_gate_up(axh_context *ctx, const void *gate_codes,
   const uint64_t slots = (uint64_t)n_tokens * top_k;
   if (slots > 65535u) return bad("at most 65535 slots: prompts take the matmul form");
   const uint32_t nblk = cols / 32u;
-  const MatvecPlan p = plan_matvec(n_rows, nblk, 1, 2, (uint32_t)slots);
+  const MatvecPlan p = plan_matvec(n_rows, nblk, 1, 8, 2, (uint32_t)slots);
   const uint32_t words[] = {n_rows, nblk, p.uw, p.batches, top_k, n_experts};
   void *bufs[] = {mut(gate_codes), mut(gate_scales), mut(up_codes), mut(up_scales),
                   mut(x),          mut(experts),     h};
@@ -388,7 +396,7 @@ axh_status axh_mxfp4_expert_down(axh_context *ctx, const void *codes, const void
   if ((uint64_t)n_tokens * top_k > 65535u)
     return bad("at most 65535 slots: prompts take the matmul form");
   const uint32_t nblk = cols / 32u;
-  const MatvecPlan p = plan_matvec(n_rows, nblk, top_k, 1, n_tokens);
+  const MatvecPlan p = plan_matvec(n_rows, nblk, top_k, 4, 1, n_tokens);
   const uint32_t words[] = {n_rows, nblk, p.uw, p.batches, top_k, n_experts};
   void *bufs[] = {mut(codes), mut(scales), mut(h), mut(experts), mut(weights), y};
   return launch(ctx, kMatvec, "axh_mxfp4_expert_down_l" + std::to_string(p.lanes), p.wgs, n_tokens,
