@@ -359,40 +359,54 @@ AXH_ROUTE_N(8)
 AXH_ROUTE_N(16)
 
 // ---------------------------------------------------------------------------
-// The order of slots by expert: a stable counting sort in one workgroup.  Slot
-// i is choice i % top_k of token i / top_k.  Wave w takes a contiguous part of
-// the slots; counts per wave and expert, their prefix sums over (expert, wave),
-// then each wave hands out places in slot order: within 64 slots, the lanes
-// with the same expert are found by one ballot per bit of the expert's index.
+// The order of slots by expert: a stable counting sort.  Slot i is choice
+// i % top_k of token i / top_k.  A workgroup gives a contiguous chunk of the
+// slots their places, a wave of it a contiguous part of the chunk; it counts the
+// experts of the slots before its chunk, of each wave's part and after the chunk,
+// so that no workgroup waits for another.  Within 64 slots, the lanes with the
+// same expert are found by one ballot per bit of the expert's index: these are
+// the most of the work, which is why the slots are shared out to workgroups.
 // plan: offsets[n_experts + 1], padded to 16 words, then the slots.
+//   3.9 us for 2000 slots of 40 experts, 7.0 us for 16384 of 32 (12.9 in one workgroup
+// with a load at a time).
 // ---------------------------------------------------------------------------
 extern "C" __global__ void __launch_bounds__(1024) axh_expert_plan(const int32_t *experts,
                                                                   uint32_t *plan,
                                                                   uint32_t n_slots,
                                                                   uint32_t n_experts,
-                                                                  uint32_t id_bits) {
-  extern __shared__ uint32_t lds[]; // [16][n_experts] counts, then places; [16] sums
+                                                                  uint32_t id_bits,
+                                                                  uint32_t part_bits) {
+  // [16 waves, then slots before the chunk, then after it][n_experts]: counts, then
+  // the waves' places; [16] sums
+  extern __shared__ uint32_t lds[];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  uint32_t *sums = lds + 16u * n_experts;
-  for (uint32_t i = tid; i < 16u * n_experts; i += 1024u) lds[i] = 0u;
+  uint32_t *sums = lds + 18u * n_experts;
+  for (uint32_t i = tid; i < 18u * n_experts; i += 1024u) lds[i] = 0u;
   __syncthreads();
-  // a wave's part is a multiple of 64, so only the last 64 are partial
-  const uint32_t part = ((n_slots + 1023u) / 1024u) * 64u;
-  const uint32_t from = wave * part;
-  const uint32_t to = from + part < n_slots ? from + part : n_slots;
-  for (uint32_t i = from + lane; i < to; i += 64u) {
-    const uint32_t e = (uint32_t)experts[i];
-    if (e < n_experts) atomicAdd(&lds[wave * n_experts + e], 1u);
+  const uint32_t part = 1u << part_bits, chunk = 16u * part, from = blockIdx.x * chunk;
+  for (uint32_t i0 = tid; i0 < n_slots; i0 += 8192u) {
+    uint32_t e[8]; // all requested before the first is waited for
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) {
+      const uint32_t i = i0 + 1024u * k;
+      e[k] = (uint32_t)experts[i < n_slots ? i : n_slots - 1u];
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) {
+      const uint32_t i = i0 + 1024u * k;
+      const uint32_t row = i < from ? 16u : i - from < chunk ? i - from >> part_bits : 17u;
+      if (i < n_slots && e[k] < n_experts) atomicAdd(&lds[row * n_experts + e[k]], 1u);
+    }
   }
   __syncthreads();
-  // thread e: the expert's total, and its waves' counts turned into prefixes
-  uint32_t total = 0;
-  if (tid < n_experts)
-    for (uint32_t w = 0; w < 16u; ++w) {
-      const uint32_t c = lds[w * n_experts + tid];
-      lds[w * n_experts + tid] = total;
-      total += c;
-    }
+  // thread e: the expert's counts, and their total
+  uint32_t counts[18], total = 0;
+  if (tid < n_experts) {
+#pragma unroll
+    for (uint32_t w = 0; w < 18u; ++w) counts[w] = lds[w * n_experts + tid];
+#pragma unroll
+    for (uint32_t w = 0; w < 18u; ++w) total += counts[w];
+  }
   uint32_t incl = total; // inclusive prefix over the experts of this wave
 #pragma unroll
   for (uint32_t d = 1; d < 64u; d <<= 1) {
@@ -401,33 +415,53 @@ extern "C" __global__ void __launch_bounds__(1024) axh_expert_plan(const int32_t
   }
   if (lane == 63u) sums[wave] = incl;
   __syncthreads();
-  uint32_t base = 0;
-  for (uint32_t w = 0; w < wave; ++w) base += sums[w];
-  const uint32_t first = base + incl - total;
+  uint32_t first = incl - total;
+#pragma unroll
+  for (uint32_t w = 0; w < 16u; ++w) first += w < wave ? sums[w] : 0u;
   if (tid < n_experts) {
-    plan[tid] = first;
-    if (tid == n_experts - 1u) plan[n_experts] = first + total;
-    for (uint32_t w = 0; w < 16u; ++w) lds[w * n_experts + tid] += first;
+    if (blockIdx.x == 0) {
+      plan[tid] = first;
+      if (tid == n_experts - 1u) plan[n_experts] = first + total;
+    }
+    first += counts[16];
+#pragma unroll
+    for (uint32_t w = 0; w < 16u; ++w) {
+      lds[w * n_experts + tid] = first;
+      first += counts[w];
+    }
   }
   __syncthreads();
   uint32_t *order = plan + ((n_experts + 1u + 15u) & ~15u);
-  for (uint32_t i0 = from; i0 < to; i0 += 64u) {
-    const uint32_t i = i0 + lane;
-    const uint32_t e = i < to ? (uint32_t)experts[i] : 0xFFFFFFFFu;
-    const bool in = e < n_experts;
-    uint64_t same = __ballot(in);
-    for (uint32_t b = 0; b < id_bits; ++b) {
-      const bool bit = (e >> b) & 1u;
-      const uint64_t set = __ballot(bit);
-      same &= bit ? set : ~set;
+  uint32_t i0 = from + wave * part;
+  const uint32_t to = i0 + part < n_slots ? i0 + part : n_slots;
+  for (; i0 < to; i0 += 128u) { // (a part is 128 or more)
+    uint32_t e[2], lo[2], hi[2]; // lo, hi: the lanes with the same expert
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k) {
+      const uint32_t i = i0 + 64u * k + lane;
+      e[k] = i < to ? (uint32_t)experts[i] : n_experts;
+      const uint64_t in = __ballot(e[k] < n_experts);
+      lo[k] = (uint32_t)in;
+      hi[k] = (uint32_t)(in >> 32);
     }
-    if (in) {
-      const uint32_t before = __builtin_popcountll(same & ((1ull << lane) - 1ull));
-      const uint32_t at = lds[wave * n_experts + e];
-      order[at + before] = i;
-      // the last of the lanes moves the place on; the wave's LDS operations are in order
-      if ((same >> lane) == 1ull) lds[wave * n_experts + e] = at + before + 1u;
-    }
+    for (uint32_t b = 0; b < id_bits; ++b)
+#pragma unroll
+      for (uint32_t k = 0; k < 2; ++k) {
+        const uint32_t mask = 0u - (e[k] >> b & 1u);
+        const uint64_t set = __ballot(mask != 0u);
+        lo[k] &= ~((uint32_t)set ^ mask);
+        hi[k] &= ~((uint32_t)(set >> 32) ^ mask);
+      }
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k)
+      if (e[k] < n_experts) {
+        const uint32_t before = __builtin_amdgcn_mbcnt_hi(hi[k], __builtin_amdgcn_mbcnt_lo(lo[k], 0u));
+        const uint32_t at = lds[wave * n_experts + e[k]] + before;
+        if (at < n_slots) order[at] = i0 + 64u * k + lane; // (not less only if experts change meanwhile)
+        // the last of the lanes moves the place on; the wave's LDS operations are in order
+        if (before + 1u == (uint32_t)(__builtin_popcount(lo[k]) + __builtin_popcount(hi[k])))
+          lds[wave * n_experts + e[k]] = at + 1u;
+      }
   }
 }
 

@@ -163,15 +163,34 @@ struct Tile {
   bool real;
 };
 
-// Workgroup -> tile.  Consecutive workgroups go to the eight XCDs in turn; each
-// XCD is given a contiguous part of the tiles, rows fastest for expert layers
-// (the tiles of one group of columns share X), columns fastest otherwise.
-template <Mode M, int BN> __device__ __forceinline__ Tile tile_of(const Args &a) {
-  const uint32_t total = gridDim.x, id = blockIdx.x;
+// Number k of a contiguous part for each of the eight XCDs, to which consecutive
+// workgroups go in turn: tiles that share data then share an L2.
+__device__ __forceinline__ uint32_t by_xcd(uint32_t id, uint32_t total) {
   const uint32_t per = total / 8u, rest = total % 8u, xcd = id % 8u;
-  const uint32_t t = xcd * per + (xcd < rest ? xcd : rest) + id / 8u;
+  return xcd * per + (xcd < rest ? xcd : rest) + id / 8u;
+}
+
+// Inclusive prefix sum over the wave.
+__device__ __forceinline__ uint32_t prefix(uint32_t v, uint32_t lane) {
+#pragma unroll
+  for (uint32_t d = 1; d < 64u; d <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// Workgroup -> tile, columns fastest in dense products and rows fastest in expert
+// layers, where the tiles of one group of columns share X.
+//   How many tiles an expert layer has is in the plan only; the grid is an upper
+// bound, and the XCDs share the real ones (sharing the grid's left the last XCDs
+// without work: 333 tokens, 6 of 40 experts, 1312 x 736, 26.1 us in place of 15.7).  Every wave finds the expert of its tile: each lane sums up
+// the tiles of its experts, and for more than 64 experts a second step looks through
+// those of the lane that was found.
+template <Mode M, int BN> __device__ __forceinline__ Tile tile_of(const Args &a) {
   Tile r;
   if constexpr (M == kDense) {
+    const uint32_t t = by_xcd(blockIdx.x, gridDim.x);
     const uint32_t cols = (a.n_cols + BN - 1u) / BN;
     r.m = t / cols;
     r.n0 = (t - r.m * cols) * BN;
@@ -180,47 +199,60 @@ template <Mode M, int BN> __device__ __forceinline__ Tile tile_of(const Args &a)
     r.expert = 0;
     r.real = true;
   } else {
-    const uint32_t nt = t / a.row_tiles;
-    r.m = t - nt * a.row_tiles;
-    // the expert whose tiles of BN columns hold number nt: every wave looks
-    // through the offsets, 64 experts at a time
-    const uint32_t lane = threadIdx.x & 63u;
-    uint32_t before = 0;
-    r.real = false;
-    r.n0 = r.count = r.first = r.expert = 0;
-    for (uint32_t e0 = 0; e0 < a.n_experts; e0 += 64u) {
-      const uint32_t e = e0 + lane;
-      const uint32_t lo = a.plan[e < a.n_experts ? e : a.n_experts];
-      const uint32_t hi = a.plan[e < a.n_experts ? e + 1u : a.n_experts];
-      const uint32_t tiles = (hi - lo + BN - 1u) / BN;
-      uint32_t incl = tiles;
-#pragma unroll
-      for (uint32_t d = 1; d < 64u; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)incl, d);
-        if (lane >= d) incl += o;
-      }
-      const uint32_t excl = before + incl - tiles;
-      const uint64_t at = __ballot(nt >= excl && nt < excl + tiles);
-      if (at) {
-        const int who = __builtin_ctzll(at);
-        const uint32_t k = (nt - (uint32_t)__builtin_amdgcn_readlane((int)excl, who)) * BN;
-        const uint32_t l = (uint32_t)__builtin_amdgcn_readlane((int)lo, who);
-        const uint32_t h = (uint32_t)__builtin_amdgcn_readlane((int)hi, who);
-        r.expert = e0 + (uint32_t)who;
-        r.first = l + k;
-        r.count = h - l - k;
-        r.real = true;
-        break;
-      }
-      before += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+    const uint32_t lane = threadIdx.x & 63u, slots = a.n_x * a.x_div;
+    const uint32_t per = (a.n_experts + 63u) / 64u;
+    auto offset = [&](uint32_t e) { // kept in range: see slot_at
+      const uint32_t o = a.plan[e < a.n_experts ? e : a.n_experts];
+      return o < slots ? o : slots;
+    };
+    auto tiles_of = [](uint32_t lo, uint32_t hi) {
+      return hi > lo ? (hi - lo + BN - 1u) / BN : 0u;
+    };
+    uint32_t e0 = lane * per, lo = offset(e0), hi = lo, tiles = 0;
+#pragma unroll 4
+    for (uint32_t j = 0; j < per; ++j) {
+      const uint32_t next = offset(e0 + j + 1u);
+      tiles += tiles_of(hi, next);
+      hi = next;
     }
+    uint32_t incl = prefix(tiles, lane);
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63) * a.row_tiles;
+    r.real = blockIdx.x < total;
+    r.m = r.n0 = r.count = r.first = r.expert = 0;
+    if (!r.real) return r;
+    const uint32_t t = by_xcd(blockIdx.x, total);
+    uint32_t nt = t / a.row_tiles;
+    r.m = t - nt * a.row_tiles;
+    int who = __builtin_ctzll(__ballot(nt < incl));
+    nt -= (uint32_t)__builtin_amdgcn_readlane((int)(incl - tiles), who);
+    if (per > 1u) {
+      const uint32_t of = (uint32_t)who * per;
+      e0 = of + (lane < per ? lane : per);
+      lo = offset(e0);
+      hi = offset(e0 + (lane < per ? 1u : 0u));
+      tiles = tiles_of(lo, hi);
+      incl = prefix(tiles, lane);
+      who = __builtin_ctzll(__ballot(nt < incl) | 1ull << 63);
+      nt -= (uint32_t)__builtin_amdgcn_readlane((int)(incl - tiles), who);
+    }
+    r.expert = (uint32_t)__builtin_amdgcn_readlane((int)e0, who);
+    r.expert = r.expert < a.n_experts ? r.expert : a.n_experts - 1u;
+    const uint32_t l = (uint32_t)__builtin_amdgcn_readlane((int)lo, who) + nt * BN;
+    const uint32_t h = (uint32_t)__builtin_amdgcn_readlane((int)hi, who);
+    r.first = l;
+    r.count = h - l;
+    r.real = l < h;
   }
   if (r.count > (uint32_t)BN) r.count = BN;
   return r;
 }
 
-__device__ __forceinline__ const uint32_t *plan_order(const Args &a) {
-  return a.plan + ((a.n_experts + 1u + 15u) & ~15u);
+// The slot at place p of the plan's order.  Kept in range, as the offsets are: a plan
+// that was overwritten gives wrong rows, but no access outside the buffers.
+__device__ __forceinline__ uint32_t slot_at(const Args &a, uint32_t p) {
+  const uint32_t slot = a.plan[((a.n_experts + 1u + 15u) & ~15u) + p];
+  const uint32_t last = a.n_x * a.x_div - 1u;
+  return slot < last ? slot : last;
 }
 
 // Finishes four rows r .. r + 3 of a column (not packed).
@@ -264,7 +296,7 @@ __device__ __forceinline__ void ksplit_body(const Args &a, uint8_t *lds) {
   const __amdgpu_buffer_rsrc_t xc = rsrc(a.xc + xbase * row_bytes, xrows * row_bytes);
   const __amdgpu_buffer_rsrc_t xs = rsrc(a.xs + xbase * nblk, xrows * nblk);
   auto slot_of = [&](uint32_t j) {
-    return M == kDense ? t.n0 + j : plan_order(a)[t.first + (j < t.count ? j : 0u)];
+    return M == kDense ? t.n0 + j : slot_at(a, t.first + (j < t.count ? j : 0u));
   };
   auto xrow_of = [&](uint32_t j) { return M == kDense ? j : slot_of(j) / a.x_div; };
 
@@ -474,7 +506,7 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   constexpr int kSRows = (BM + BN + 64 * NW - 1) / (64 * NW); // rows of scales per lane
   constexpr uint32_t kBuf = (BM + BN) * 128u, kSBuf = kSRows * 64u * NW * 16u;
   constexpr int kLoads = (BM + BN) / 8 / NW; // per wave and step; rows of A first
-  constexpr int kALoads = BM / 8 / NW;
+  constexpr int kALoads = BM / 8 / NW, kHalf = kLoads / 2;
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads per wave");
   static_assert(NW % 2 == 0, "the rows of a lane's loads are alike mod 16");
   static_assert(M != kGateUp || MI % 2 == 0, "gate and up rows in one wave");
@@ -497,23 +529,30 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   const __amdgpu_buffer_rsrc_t xc = rsrc(a.xc + xbase * row_bytes, xrows * row_bytes);
   // row of X of column j of the tile, and the row of y that it gives
   auto slot_of = [&](uint32_t j) {
-    return M == kDense ? t.n0 + j : plan_order(a)[t.first + (j < t.count ? j : 0u)];
+    return M == kDense ? t.n0 + j : slot_at(a, t.first + (j < t.count ? j : 0u));
   };
-  auto xrow_of = [&](uint32_t j) { return M == kDense ? j : slot_of(j) / a.x_div; };
 
   // this lane's part of each load of codes: row 8 * (load * NW + wave) + lane / 8
   const uint32_t l8 = lane >> 3, piece = (lane & 7u) ^ ((4u * wave + (l8 >> 1)) & 7u);
-  uint32_t off[kLoads];
+  // The columns' slots are requested first and used behind the requests of A below:
+  // they are the end of a chain of loads, expert, slot, row of X.
+  uint32_t off[kLoads], slot[kLoads - kALoads], sslot[kSRows];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    if (i < kALoads) {
-      const uint32_t r = 8u * (i * NW + wave) + l8;
-      const uint32_t row = M == kGateUp ? (r >> 6) * 32u + (r & 31u) : r;
-      off[i] = row * row_bytes + piece * 16u;
-    } else {
-      const uint32_t j = 8u * ((i - kALoads) * NW + wave) + l8;
-      off[i] = j < t.count ? xrow_of(j) * row_bytes + piece * 16u : kFar;
-    }
+  for (int i = kALoads; i < kLoads; ++i) {
+    const uint32_t j = 8u * ((i - kALoads) * NW + wave) + l8;
+    slot[i - kALoads] = slot_of(j);
+  }
+#pragma unroll
+  for (int i = 0; i < kSRows; ++i) {
+    const uint32_t r = 64u * NW * i + threadIdx.x, j = r < (uint32_t)BM ? 0u : r - BM;
+    sslot[i] = slot_of(j < t.count ? j : t.count - 1u);
+  }
+  auto xrow = [&](uint32_t s) { return M == kDense ? s - t.n0 : s / a.x_div; };
+#pragma unroll
+  for (int i = 0; i < kALoads; ++i) {
+    const uint32_t r = 8u * (i * NW + wave) + l8;
+    const uint32_t row = M == kGateUp ? (r >> 6) * 32u + (r & 31u) : r;
+    off[i] = row * row_bytes + piece * 16u;
   }
   const uint32_t steps = (nblk + 7u) / 8u;
   // load i of step s into buffer buf; steps past the end: zeros
@@ -525,6 +564,22 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kALoads ? (up ? uc : wc) : xc, (lds_void_t *)to,
                                              16, (int)(in ? off[i] + s * 128u : kFar), 0, 0, 0);
   };
+
+  // The first loads: A of the steps 0 .. NBUF - 2, then their X, then half of step
+  // NBUF - 1's.  The waits count on every load of a step being older than all of the
+  // steps from NBUF - 1 on.
+  static_assert(NBUF <= 3, "else step 1's X is younger than step 2's A");
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (uint32_t st = 0; st + 1u < NBUF; ++st)
+#pragma unroll
+    for (int i = 0; i < kALoads; ++i) request(st, st, i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = kALoads; i < kLoads; ++i) {
+    const uint32_t j = 8u * ((i - kALoads) * NW + wave) + l8;
+    off[i] = j < t.count ? xrow(slot[i - kALoads]) * row_bytes + piece * 16u : kFar;
+  }
 
   // scales: lane (64 * NW * i + thread) takes a row of A or of B (rows that there
   // are not: the last one's, whose products are not stored)
@@ -538,8 +593,7 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
       const bool up = M == kGateUp && ((r >> 5) & 1u);
       sbase[i] = (up ? a.us : a.ws) + wat + (uint64_t)row * nblk;
     } else { // (lanes past the rows of B repeat its last one)
-      const uint32_t j = r - BM;
-      sbase[i] = a.xs + (xbase + xrow_of(j < t.count ? j : t.count - 1u)) * nblk;
+      sbase[i] = a.xs + (xbase + xrow(sslot[i])) * nblk;
     }
   }
   // the scales of blocks 16 p .. 16 p + 15, read inside the row: at its end from
@@ -619,7 +673,7 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   // What goes among a part's products: the next part's fragments f (part k of
   // buffer from) and the requests [begin, end) of step s into buffer `to`.  The
   // compiler keeps reads and requests in this order, both being accesses to LDS.
-  constexpr int kHalf = kLoads / 2, kReads = MI + NI;
+  constexpr int kReads = MI + NI;
   auto loads = [&](Frags &f, int k, uint32_t from, uint32_t s, uint32_t to, int begin, int end) {
     const int n = end - begin;
 #pragma unroll
@@ -681,13 +735,15 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
 
   get_scales(0);
 #pragma unroll
-  for (uint32_t s = 0; s < NBUF; ++s)
+  for (uint32_t st = 0; st + 1u < NBUF; ++st)
 #pragma unroll
-    for (int i = 0; i < (s + 1u < NBUF ? kLoads : kHalf); ++i) request(s, s, i);
+    for (int i = kALoads; i < kLoads; ++i) request(st, st, i);
+#pragma unroll
+  for (int i = 0; i < kHalf; ++i) request(NBUF - 1u, NBUF - 1u, i);
   put_scales(0);
   get_scales(1);
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 2) * kLoads + kHalf +
-                                                                  kSRows)
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
+                   (NBUF - 2) * (kLoads - kALoads) + kHalf + kSRows) // (all younger than step 0)
                : "memory");
   read_frags(f0, 0, 0);
   read_scales(c0, 0);
@@ -801,73 +857,73 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   const Args a{wc, ws, uc, us, xc, xs, plan, y, ysc, n_rows, nblk, 0u, n_x, x_div, n_experts,     \
                row_tiles}
 
-// K-split kernels: kRows rows, NW waves, NB buffers of each.
-#define AXH_MX_KSPLIT(NAME, TN, T, ROWS, NW, NB)                                                  \
-  extern "C" __global__ void __launch_bounds__(64 * NW)                                           \
-      axh_mxfp4_matmul_##NAME##_##TN(AXH_MX_DENSE_ARGS) {                                         \
-    extern __shared__ __align__(16) uint8_t ring[];                                               \
-    AXH_MX_DENSE_UNPACK;                                                                          \
-    ksplit_body<kDense, T, false, ROWS, NW, NB>(a, ring);                                         \
-  }                                                                                               \
-  extern "C" __global__ void __launch_bounds__(64 * NW)                                           \
-      axh_mxfp4_expert_matmul_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {                                 \
-    extern __shared__ __align__(16) uint8_t ring[];                                               \
-    AXH_MX_EXPERT_UNPACK;                                                                         \
-    ksplit_body<kGrouped, T, false, ROWS, NW, NB>(a, ring);                                       \
-  }
-#define AXH_MX_KSPLIT_GU(NAME, TN, T, PACKED, NW, NB)                                             \
-  extern "C" __global__ void __launch_bounds__(64 * NW)                                           \
-      axh_mxfp4_expert_gate_up_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {                                \
-    extern __shared__ __align__(16) uint8_t ring[];                                               \
-    AXH_MX_EXPERT_UNPACK;                                                                         \
-    ksplit_body<kGateUp, T, PACKED, 32, NW, NB>(a, ring);                                         \
-  }
-#define AXH_MX_KSPLIT_N(NAME, ROWS, NW, NB)        \
-  AXH_MX_KSPLIT(NAME, f32, TF32, ROWS, NW, NB)     \
-  AXH_MX_KSPLIT(NAME, f16, TF16, ROWS, NW, NB)     \
-  AXH_MX_KSPLIT(NAME, bf16, TBF16, ROWS, NW, NB)
-#define AXH_MX_KSPLIT_GU_N(NAME, NW, NB)                 \
-  AXH_MX_KSPLIT_GU(NAME, f32, TF32, false, NW, NB)       \
-  AXH_MX_KSPLIT_GU(NAME, f16, TF16, false, NW, NB)       \
-  AXH_MX_KSPLIT_GU(NAME, bf16, TBF16, false, NW, NB)     \
-  AXH_MX_KSPLIT_GU(NAME, mxfp4, TF32, true, NW, NB)
-AXH_MX_KSPLIT_N(k16, 16, 8, 3)
-AXH_MX_KSPLIT_N(k32, 32, 8, 2)
-AXH_MX_KSPLIT_GU_N(k32, 4, 3)
+#define AXH_MX_TYPES(KERNEL, ...)  \
+  KERNEL(f32, TF32, __VA_ARGS__)   \
+  KERNEL(f16, TF16, __VA_ARGS__)   \
+  KERNEL(bf16, TBF16, __VA_ARGS__)
 
-// Tile kernels.
-#define AXH_MX_TILE(NAME, TN, T, BM, BN, WM, WN, NBUF, WPE)                                             \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN)                                      \
-      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                                              \
-      axh_mxfp4_matmul_##NAME##_##TN(AXH_MX_DENSE_ARGS) {                                         \
-    extern __shared__ __align__(16) uint8_t tile[];                                                       \
-    AXH_MX_DENSE_UNPACK;                                                                          \
-    tile_body<kDense, T, false, BM, BN, WM, WN, NBUF>(a, tile);                                         \
-  }                                                                                               \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN)                                      \
-      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                                              \
-      axh_mxfp4_expert_matmul_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {                                 \
-    extern __shared__ __align__(16) uint8_t tile[];                                                       \
-    AXH_MX_EXPERT_UNPACK;                                                                         \
-    tile_body<kGrouped, T, false, BM, BN, WM, WN, NBUF>(a, tile);                                       \
+// K-split kernels: NAME, rows, waves, buffers of a wave.
+#define AXH_MX_KSPLIT_DENSE(TN, T, NAME, ROWS, NW, NB)           \
+  extern "C" __global__ void __launch_bounds__(64 * NW)          \
+      axh_mxfp4_matmul_##NAME##_##TN(AXH_MX_DENSE_ARGS) {        \
+    extern __shared__ __align__(16) uint8_t ring[];              \
+    AXH_MX_DENSE_UNPACK;                                         \
+    ksplit_body<kDense, T, false, ROWS, NW, NB>(a, ring);        \
   }
-#define AXH_MX_TILE_GU(NAME, TN, T, PACKED, BM, BN, WM, WN, NBUF, WPE)                                  \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN)                                      \
-      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                                              \
-      axh_mxfp4_expert_gate_up_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {                                \
-    extern __shared__ __align__(16) uint8_t tile[];                                                       \
-    AXH_MX_EXPERT_UNPACK;                                                                         \
-    tile_body<kGateUp, T, PACKED, BM, BN, WM, WN, NBUF>(a, tile);                                       \
+#define AXH_MX_KSPLIT_EXPERT(TN, T, NAME, ROWS, NW, NB)          \
+  extern "C" __global__ void __launch_bounds__(64 * NW)          \
+      axh_mxfp4_expert_matmul_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {\
+    extern __shared__ __align__(16) uint8_t ring[];              \
+    AXH_MX_EXPERT_UNPACK;                                        \
+    ksplit_body<kGrouped, T, false, ROWS, NW, NB>(a, ring);      \
   }
-#define AXH_MX_TILE_N(NAME, BM, BN, WM, WN, NBUF, WPE)                   \
-  AXH_MX_TILE(NAME, f32, TF32, BM, BN, WM, WN, NBUF, WPE)                \
-  AXH_MX_TILE(NAME, f16, TF16, BM, BN, WM, WN, NBUF, WPE)                \
-  AXH_MX_TILE(NAME, bf16, TBF16, BM, BN, WM, WN, NBUF, WPE)              \
-  AXH_MX_TILE_GU(NAME, f32, TF32, false, BM, BN, WM, WN, NBUF, WPE)      \
-  AXH_MX_TILE_GU(NAME, f16, TF16, false, BM, BN, WM, WN, NBUF, WPE)      \
-  AXH_MX_TILE_GU(NAME, bf16, TBF16, false, BM, BN, WM, WN, NBUF, WPE)    \
-  AXH_MX_TILE_GU(NAME, mxfp4, TF32, true, BM, BN, WM, WN, NBUF, WPE)
-AXH_MX_TILE_N(t64x64, 64, 64, 1, 2, 3, 1)
-AXH_MX_TILE_N(t64x128, 64, 128, 1, 4, 3, 2)
-AXH_MX_TILE_N(t128x128, 128, 128, 2, 2, 2, 2)
-AXH_MX_TILE_N(t256x256, 256, 256, 2, 4, 2, 2)
+#define AXH_MX_KSPLIT_GATE_UP(TN, T, NAME, PACKED, NW, NB)         \
+  extern "C" __global__ void __launch_bounds__(64 * NW)            \
+      axh_mxfp4_expert_gate_up_##NAME##_##TN(AXH_MX_EXPERT_ARGS) { \
+    extern __shared__ __align__(16) uint8_t ring[];                \
+    AXH_MX_EXPERT_UNPACK;                                          \
+    ksplit_body<kGateUp, T, PACKED, 32, NW, NB>(a, ring);          \
+  }
+AXH_MX_TYPES(AXH_MX_KSPLIT_DENSE, k16, 16, 8, 3)
+AXH_MX_TYPES(AXH_MX_KSPLIT_DENSE, k32, 32, 8, 2)
+AXH_MX_TYPES(AXH_MX_KSPLIT_EXPERT, k32, 32, 8, 2)
+AXH_MX_TYPES(AXH_MX_KSPLIT_GATE_UP, k32, false, 4, 3)
+AXH_MX_KSPLIT_GATE_UP(mxfp4, TF32, k32, true, 4, 3)
+
+// Tile kernels: NAME, rows and columns of the tile, waves along both, buffers, waves
+// of a SIMD.
+#define AXH_MX_TILE_DENSE(TN, T, NAME, BM, BN, WM, WN, NBUF, WPE) \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN)      \
+      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))              \
+      axh_mxfp4_matmul_##NAME##_##TN(AXH_MX_DENSE_ARGS) {         \
+    extern __shared__ __align__(16) uint8_t tile[];               \
+    AXH_MX_DENSE_UNPACK;                                          \
+    tile_body<kDense, T, false, BM, BN, WM, WN, NBUF>(a, tile);   \
+  }
+#define AXH_MX_TILE_EXPERT(TN, T, NAME, BM, BN, WM, WN, NBUF, WPE) \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN)       \
+      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))               \
+      axh_mxfp4_expert_matmul_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {  \
+    extern __shared__ __align__(16) uint8_t tile[];                \
+    AXH_MX_EXPERT_UNPACK;                                          \
+    tile_body<kGrouped, T, false, BM, BN, WM, WN, NBUF>(a, tile);  \
+  }
+#define AXH_MX_TILE_GATE_UP(TN, T, NAME, PACKED, BM, BN, WM, WN, NBUF, WPE) \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN)                \
+      __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                        \
+      axh_mxfp4_expert_gate_up_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {          \
+    extern __shared__ __align__(16) uint8_t tile[];                         \
+    AXH_MX_EXPERT_UNPACK;                                                   \
+    tile_body<kGateUp, T, PACKED, BM, BN, WM, WN, NBUF>(a, tile);           \
+  }
+#define AXH_MX_TILE_EXPERTS(NAME, ...)                        \
+  AXH_MX_TYPES(AXH_MX_TILE_EXPERT, NAME, __VA_ARGS__)         \
+  AXH_MX_TYPES(AXH_MX_TILE_GATE_UP, NAME, false, __VA_ARGS__) \
+  AXH_MX_TILE_GATE_UP(mxfp4, TF32, NAME, true, __VA_ARGS__)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t64x64, 64, 64, 1, 2, 3, 1)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t64x128, 64, 128, 1, 4, 3, 2)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t128x128, 128, 128, 2, 2, 2, 2)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t256x256, 256, 256, 2, 4, 2, 2)
+AXH_MX_TILE_EXPERTS(t128x64, 128, 64, 2, 2, 3, 2)
+AXH_MX_TILE_EXPERTS(t128x128, 128, 128, 2, 2, 2, 2)
+AXH_MX_TILE_EXPERTS(t256x256, 256, 256, 2, 4, 2, 2)

@@ -105,43 +105,59 @@ MatvecPlan plan_matvec(uint32_t n_rows, uint32_t nblk, uint32_t picks, uint32_t 
 }
 
 // ---- matmul kernels -----------------------------------------------------------
+// A kind's tile and launch; keep in sync with mx_matmul.hip.
 struct MatmulKind {
   const char *name;
-  uint32_t rows, cols;   // a workgroup's outputs
-  uint32_t rows_gu;      // rows of each matrix (gate/up), 0 where there is none
-  uint32_t threads, threads_gu;
-  uint32_t lds, lds_gu;
+  uint32_t rows, cols; // a workgroup's outputs (gate/up: half of the rows)
+  uint32_t threads, lds;
 };
-// From the largest tile to the smallest; keep in sync with mx_matmul.hip.
-constexpr MatmulKind kTiles[] = {
-    {"t256x256", 256, 256, 128, 512, 512, 147456, 147456},
-    {"t128x128", 128, 128, 64, 256, 256, 73728, 73728},
-    {"t64x128", 64, 128, 32, 256, 256, 81920, 81920},
-    {"t64x64", 64, 64, 32, 128, 128, 53248, 53248},
-};
-constexpr MatmulKind kSplit32 = {"k32", 32, 32, 32, 512, 256, 131072, 147456};
-constexpr MatmulKind kSplit16 = {"k16", 16, 32, 0, 512, 0, 147456, 0};
+constexpr MatmulKind k256x256 = {"t256x256", 256, 256, 512, 147456};
+constexpr MatmulKind k128x128 = {"t128x128", 128, 128, 256, 73728};
+constexpr MatmulKind k128x64 = {"t128x64", 128, 64, 256, 81920};
+constexpr MatmulKind k64x128 = {"t64x128", 64, 128, 256, 81920};
+constexpr MatmulKind k64x64 = {"t64x64", 64, 64, 128, 53248};
+constexpr MatmulKind kSplit32 = {"k32", 32, 32, 512, 131072};
+constexpr MatmulKind kSplit32GateUp = {"k32", 64, 32, 256, 147456};
+constexpr MatmulKind kSplit16 = {"k16", 16, 32, 512, 147456};
 constexpr uint32_t kTileMinBlocks = 16; // the tiles read 16 scales of a row at once
-constexpr uint32_t kFullGrid = 200, kLongBlocks = 256;
 
+// The largest tile that gives most of the 256 CUs one (and is not mostly empty): a
+// larger one reads less, but what has no tile waits.  14336 x 4096, us: 512
+// columns 128x128 31.9, 256x256 (112 tiles) 34.3, 64x64 51.8; 1024 columns 45.2 with
+// 256x256, 58.6 with 128x128; 256 columns 128x128 20.9, 64x128 22.6; 96 columns 64x128
+// 13.5, 128x128 18.9.  Where even 64x64 gives too few, the K-split kernel, if its own
+// tiles fit one round of workgroups (4096 x 4096, 64 columns: 6.6 against 8.7; 96
+// columns, 384 tiles: 64x64 9.2, K-split 11.7) or K is long (4096 x 14336, 128 columns:
+// 26.9 against 28.7), and in the latter case with half the rows if those fit too
+// (4096 x 14336, 32 columns: 14.0 against 16.3; 8192 x 8192, 64 columns: 64x64 18.6,
+// K-split 20.4).
 const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
   auto grid = [&](const MatmulKind &k) {
     return (uint64_t)div_up(n_rows, k.rows) * div_up(batch, k.cols);
   };
   if (nblk < kTileMinBlocks) return kSplit32;
-  for (const MatmulKind &k : kTiles)
-    if (grid(k) >= kFullGrid && (batch > k.cols / 2u || k.cols == 64u)) return k;
-  if (grid(kSplit32) <= 256u || nblk >= kLongBlocks)
-    return grid(kSplit16) <= 256u && nblk >= kLongBlocks ? kSplit16 : kSplit32;
-  return kTiles[3];
+  for (const MatmulKind *k : {&k256x256, &k128x128, &k64x128})
+    if (grid(*k) >= 200u && batch > k->cols / 2u) return *k;
+  if (grid(k64x64) >= 200u) return k64x64;
+  const bool is_long = nblk >= 320u;
+  if (grid(kSplit32) > 256u && !is_long) return k64x64;
+  return is_long && grid(kSplit16) <= 256u ? kSplit16 : kSplit32;
 }
 
-const MatmulKind &expert_kind(uint64_t slots, uint32_t n_experts, uint32_t nblk) {
+// By the mean number of columns of an expert: tiles of 64 columns while most experts
+// have one of them, of 256 where an expert's outputs are many, so that such tiles are
+// mostly full and still many.  Gate and up / down, us.  40 experts, 1312 x 736, mean 50:
+// 128x64 15.7 / 10.4, 128x128 18.8 / 12.4.  64 experts, 2048 x 1408: mean 32: 46.5 / 27.1,
+// 55.9 / 29.5; mean 64: 58.7 / 38.1, 57.5 / 33.3; mean 256: 128x128 114 / 71, 256x256 134 /
+// 78; mean 512: 190 / 117, 189 / 107; mean 1024: 340 / 251, 332 / 219.  8 experts, 4096 x
+// 14336: mean 75: 124 / 65, 167 / 97; mean 175: 234 / 89, 186 / 104; mean 256: 322 / 159,
+// 269 / 121.
+const MatmulKind &expert_kind(uint32_t n_rows, uint32_t nblk, uint64_t slots, uint32_t n_experts,
+                              bool gate_up) {
   const uint64_t mean = slots / n_experts;
-  if (nblk < kTileMinBlocks || mean <= 16u) return kSplit32;
-  if (mean >= 192u) return kTiles[0];
-  if (mean >= 96u) return kTiles[1];
-  return kTiles[3];
+  if (nblk < kTileMinBlocks) return gate_up ? kSplit32GateUp : kSplit32;
+  if (mean <= 52u) return k128x64;
+  return mean >= 160u && mean * n_rows >= 1u << 20 ? k256x256 : k128x128;
 }
 
 // Shared checks of the expert products for prompts.
@@ -162,16 +178,14 @@ axh_status expert_launch(axh_context *ctx, const char *op, const char *type, boo
                          uint32_t x_div, uint64_t slots, uint32_t n_experts, void *stream) {
   if ((uint64_t)n_x * (cols / 2u) >= kMaxBuffer)
     return bad("the activations' codes must be below 2 GiB");
-  const MatmulKind &k = expert_kind(slots, n_experts, cols / 32u);
+  const MatmulKind &k = expert_kind(n_rows, cols / 32u, slots, n_experts, gate_up);
   // the experts' last tiles are partial: at most so many tiles in all
   const uint64_t active = std::min<uint64_t>(n_experts, slots);
   const uint64_t tiles = active + (slots - active) / k.cols;
-  const uint32_t rows = gate_up ? k.rows_gu : k.rows;
-  const uint32_t row_tiles = div_up(n_rows, rows);
+  const uint32_t row_tiles = div_up(n_rows, gate_up ? k.rows / 2u : k.rows);
   const uint32_t words[] = {n_rows, cols / 32u, n_x, x_div, n_experts, row_tiles};
   return launch(ctx, kMatmul, std::string("axh_mxfp4_") + op + "_" + k.name + "_" + type,
-                tiles * row_tiles, 1, gate_up ? k.threads_gu : k.threads,
-                gate_up ? k.lds_gu : k.lds, bufs, 9, words, 6, stream);
+                tiles * row_tiles, 1, k.threads, k.lds, bufs, 9, words, 6, stream);
 }
 
 } // namespace
@@ -415,10 +429,14 @@ axh_status axh_expert_plan(axh_context *ctx, const int32_t *experts, void *plan,
   if (!aligned(experts, 4) || !aligned(plan, 4)) return bad("experts and plan must be 4-byte aligned");
   uint32_t bits = 0;
   while ((1u << bits) < n_experts) ++bits;
-  const uint32_t words[] = {n_tokens * top_k, n_experts, bits};
+  const uint32_t slots = n_tokens * top_k;
+  // a chunk of 2048 slots each, or more, so that there are at most 128
+  uint32_t part_bits = 7;
+  while ((uint64_t)slots >> part_bits > 16u * 128u) ++part_bits;
+  const uint32_t words[] = {slots, n_experts, bits, part_bits};
   void *bufs[] = {mut(experts), plan};
-  return launch(ctx, kElem, "axh_expert_plan", 1, 1, 1024, (16u * n_experts + 16u) * 4u, bufs, 2,
-                words, 3, stream);
+  return launch(ctx, kElem, "axh_expert_plan", div_up(slots, 16ull << part_bits), 1, 1024,
+                (18u * n_experts + 16u) * 4u, bufs, 2, words, 4, stream);
 }
 
 axh_status axh_mxfp4_expert_gate_up_matmul(axh_context *ctx, const void *gate_codes,

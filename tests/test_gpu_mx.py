@@ -264,6 +264,34 @@ def test_matmul(ctx, dev, axc, rows, cols, batch, t):
     assert (np.abs(y - exact) <= bound).all()
 
 
+def test_matmul_of_many_tiles_is_that_of_few(ctx, dev, axc):
+    """More workgroups than the chip holds at once, and a long K: every column is the
+    one that calls with fewer columns, on other kernels, give."""
+    rows, cols, batch = 8192, 8192, 1024
+    _say(f"matmul {rows}x{cols} b{batch} in parts")
+    rng = np.random.default_rng(5)
+    wc = rng.integers(0, 256, rows * cols // 2, dtype=np.uint8)
+    xc = rng.integers(0, 256, batch * cols // 2, dtype=np.uint8)
+    ws = np.full(rows * cols // 32, 120, dtype=np.uint8)
+    xs = np.full(batch * cols // 32, 127, dtype=np.uint8)
+    dwc, dws, dxc, dxs = dev.up(wc), dev.up(ws), dev.up(xc), dev.up(xs)
+    # products are multiples of 2^-9 and sums below 8192 * 36 * 2^-7 < 2^12: 21 bits, so
+    # that every sum is exact, in whatever order
+    whole, names = None, set()
+    for part in (batch, 512, 256, 96, 64):
+        names.add(axc.mxfp4_matmul_kernel_name(rows, cols, part))
+        dy = dev.out(4 * rows * batch)
+        for at in range(0, batch, part):
+            n = min(part, batch - at)
+            ctx.mxfp4_matmul(dwc, dws, dxc + at * cols // 2, dxs + at * cols // 32,
+                             dy + 4 * at * rows, rows, cols, n)
+        ctx.synchronize()
+        y = dev.down(dy, 4 * rows * batch, np.float32, (batch, rows))
+        whole = y if whole is None else whole
+        assert np.array_equal(y, whole)
+    assert len(names) >= 3
+
+
 def test_matmul_special_scales(ctx, dev):
     """A NaN block reaches its row (or column) only; blocks past a row's end are
     not multiplied with the next row's."""
@@ -415,7 +443,8 @@ def _choices(seed, tokens, top_k, n_experts, holes=True):
 
 
 @pytest.mark.parametrize("tokens,top_k,n", [(1, 1, 1), (3, 2, 5), (100, 8, 64), (1000, 4, 33),
-                                            (5, 1, 1024), (2500, 6, 128), (64, 2, 2)])
+                                            (5, 1, 1024), (2500, 6, 128), (64, 2, 2),
+                                            (40000, 8, 61)])
 def test_plan(ctx, dev, axc, tokens, top_k, n):
     _say(f"plan {tokens}x{top_k} of {n}")
     e = _choices(tokens, tokens, top_k, n)

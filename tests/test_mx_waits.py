@@ -17,8 +17,9 @@ import subprocess
 import pytest
 
 OBJDUMP = shutil.which("llvm-objdump") or "/opt/rocm/llvm/bin/llvm-objdump"
-# tile -> loads of a wave and step, buffers
-TILES = {"t64x64": (8, 3), "t64x128": (6, 3), "t128x128": (8, 2), "t256x256": (8, 2)}
+# tile -> loads of a wave and step, of them of A, and buffers
+TILES = {"t64x64": (8, 4, 3), "t64x128": (6, 2, 3), "t128x64": (6, 4, 3), "t128x128": (8, 4, 2),
+         "t256x256": (8, 4, 2)}
 
 
 @pytest.fixture(scope="module")
@@ -60,12 +61,17 @@ def _in_flight(body, extra=None):
     return out
 
 
+def _named(kernels, tile):
+    named = [n for n in kernels if f"_{tile}_" in n]
+    # dense products: 3 types; expert layers: 3, gate/up: 4
+    assert len(named) == {"t64x64": 3, "t64x128": 3, "t128x64": 7}.get(tile, 10)
+    return named
+
+
 @pytest.mark.parametrize("tile", TILES)
 def test_the_next_step_has_landed_at_every_barrier(kernels, tile):
-    per_step, buffers = TILES[tile]
-    named = [n for n in kernels if f"_{tile}_" in n]
-    assert len(named) == 10  # matmul, expert matmul: 3 types; gate/up: 4
-    for name in named:
+    per_step, _, buffers = TILES[tile]
+    for name in _named(kernels, tile):
         at = _in_flight(kernels[name])
         assert len(at) >= 4, name  # prologue, two steps, the end
         # step 0 alone in the prologue: half of the last buffer's loads come in the loop
@@ -74,10 +80,37 @@ def test_the_next_step_has_landed_at_every_barrier(kernels, tile):
         assert at[-1] == 0, name  # before LDS is used for the results
 
 
+def _descriptors(body):
+    """The buffer descriptor of each load into LDS, and None for each barrier."""
+    out = []
+    for ins in body:
+        if ins.split()[0] == "s_barrier":
+            out.append(None)
+        elif ins.endswith("lds") and ins.startswith("buffer_load"):
+            out.append(re.search(r"s\[\d+:\d+\]", ins)[0])
+    return out
+
+
+@pytest.mark.parametrize("tile", TILES)
+def test_loads_come_in_the_order_that_the_waits_count_on(kernels, tile):
+    """A and X of all buffers but the last, then the last buffer's first half; in the
+    loop, second half, barrier, first half.  (With the last buffer's before X of the
+    others, the count at a barrier is the same, but the younger loads are not.)"""
+    per_step, of_a, buffers = TILES[tile]
+    step = [False] * of_a + [True] * (per_step - of_a)
+    half = per_step // 2
+    want = ([False] * of_a * (buffers - 1) + [True] * (per_step - of_a) * (buffers - 1)
+            + step[:half] + [None] + (step[half:] + [None] + step[:half]) * 2 + [None])
+    for name in _named(kernels, tile):
+        loads = _descriptors(kernels[name])
+        x = loads[of_a * (buffers - 1)]  # the first that has to be X's
+        assert [v if v is None else v == x for v in loads[:len(want)]] == want, name
+
+
 @pytest.mark.parametrize("tile", TILES)
 def test_a_longer_wait_would_be_seen(kernels, tile):
-    per_step, buffers = TILES[tile]
-    body = kernels[f"axh_mxfp4_matmul_{tile}_f32"]
+    per_step, _, buffers = TILES[tile]
+    body = kernels[_named(kernels, tile)[0]]
     assert max(_in_flight(body, extra=2)[1:]) > (buffers - 2) * per_step
 
 
