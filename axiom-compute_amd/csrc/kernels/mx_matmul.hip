@@ -499,9 +499,13 @@ __device__ __forceinline__ void ksplit_body(const Args &a, uint8_t *lds) {
 // then every wave has read its last fragments of the step, so its buffer is
 // refilled during the last part and the next step's first one, and has seen its
 // own loads of the next step land.
+//   WK groups of such waves may share the K axis, each with buffers of its own, so
+// that twice the bytes are on their way where a CU has one workgroup; the groups'
+// sums meet in LDS.
 // ---------------------------------------------------------------------------
-template <Mode M, class T, bool kPacked, int BM, int BN, int WM, int WN, int NBUF>
-__device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
+template <Mode M, class T, bool kPacked, int BM, int BN, int WM, int WN, int WK,
+          int NBUF>
+__device__ __forceinline__ void tile_body(const Args &a, uint8_t *all_lds) {
   constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
   constexpr int kSRows = (BM + BN + 64 * NW - 1) / (64 * NW); // rows of scales per lane
   constexpr uint32_t kBuf = (BM + BN) * 128u, kSBuf = kSRows * 64u * NW * 16u;
@@ -511,15 +515,22 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   static_assert(NW % 2 == 0, "the rows of a lane's loads are alike mod 16");
   static_assert(M != kGateUp || MI % 2 == 0, "gate and up rows in one wave");
   constexpr uint32_t kRows = M == kGateUp ? BM / 2 : BM; // rows of y
-  uint8_t *const slds = lds + NBUF * kBuf;
+  constexpr uint32_t kRegion = NBUF * kBuf + 2u * kSBuf;
   const uint32_t lane = threadIdx.x & 63u;
-  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t any_wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t group = WK == 1 ? 0u : any_wave / NW, wave = any_wave - group * NW;
+  const uint32_t thread = wave * 64u + lane; // of the group
+  uint8_t *const lds = all_lds + group * kRegion, *const slds = lds + NBUF * kBuf;
   const uint32_t wm = wave / WN, wn = wave % WN;
   const uint32_t half = lane >> 5, r32 = lane & 31u;
   const Tile t = tile_of<M, BN>(a);
   if (!t.real) return;
   const uint32_t row0 = t.m * kRows;
   const uint32_t nblk = a.nblk, row_bytes = nblk * 16u;
+  // the group's blocks: from kb, a multiple of 16 (two steps) but for the last group
+  const uint32_t share = WK == 1 ? nblk : (nblk + 16u * WK - 1u) / (16u * WK) * 16u;
+  const uint32_t kb = group * share, ke = kb + share < nblk ? kb + share : nblk;
+  const uint32_t kn = kb < ke ? ke - kb : 0u;
   const uint64_t wat = (uint64_t)t.expert * a.n_rows * nblk + (uint64_t)row0 * nblk;
   const uint32_t rows = a.n_rows - row0 < kRows ? a.n_rows - row0 : kRows;
   const __amdgpu_buffer_rsrc_t wc = rsrc(a.wc + wat * 16u, rows * row_bytes);
@@ -544,7 +555,7 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   }
 #pragma unroll
   for (int i = 0; i < kSRows; ++i) {
-    const uint32_t r = 64u * NW * i + threadIdx.x, j = r < (uint32_t)BM ? 0u : r - BM;
+    const uint32_t r = 64u * NW * i + thread, j = r < (uint32_t)BM ? 0u : r - BM;
     sslot[i] = slot_of(j < t.count ? j : t.count - 1u);
   }
   auto xrow = [&](uint32_t s) { return M == kDense ? s - t.n0 : s / a.x_div; };
@@ -552,12 +563,12 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   for (int i = 0; i < kALoads; ++i) {
     const uint32_t r = 8u * (i * NW + wave) + l8;
     const uint32_t row = M == kGateUp ? (r >> 6) * 32u + (r & 31u) : r;
-    off[i] = row * row_bytes + piece * 16u;
+    off[i] = row * row_bytes + (kb + piece) * 16u;
   }
-  const uint32_t steps = (nblk + 7u) / 8u;
+  const uint32_t steps = (share + 7u) / 8u;
   // load i of step s into buffer buf; steps past the end: zeros
   auto request = [&](uint32_t s, uint32_t buf, int i) {
-    const bool in = 8u * s + piece < nblk;
+    const bool in = 8u * s + piece < kn;
     const uint32_t r8 = 8u * ((i < kALoads ? i : i - kALoads) * NW + wave);
     const bool up = M == kGateUp && i < kALoads && ((r8 >> 5) & 1u);
     uint8_t *to = lds + buf * kBuf + ((i < kALoads ? 0u : (uint32_t)BM) + r8) * 128u;
@@ -578,7 +589,7 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
 #pragma unroll
   for (int i = kALoads; i < kLoads; ++i) {
     const uint32_t j = 8u * ((i - kALoads) * NW + wave) + l8;
-    off[i] = j < t.count ? xrow(slot[i - kALoads]) * row_bytes + piece * 16u : kFar;
+    off[i] = j < t.count ? xrow(slot[i - kALoads]) * row_bytes + (kb + piece) * 16u : kFar;
   }
 
   // scales: lane (64 * NW * i + thread) takes a row of A or of B (rows that there
@@ -586,7 +597,7 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   const uint8_t *sbase[kSRows];
 #pragma unroll
   for (int i = 0; i < kSRows; ++i) {
-    const uint32_t r = 64u * NW * i + threadIdx.x;
+    const uint32_t r = 64u * NW * i + thread;
     if (r < (uint32_t)BM) {
       uint32_t row = M == kGateUp ? (r >> 6) * 32u + (r & 31u) : r;
       row = row < rows ? row : rows - 1u;
@@ -601,12 +612,13 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   u32x4_t sreg[kSRows];
   const uint32_t last16 = nblk - 16u;
   auto get_scales = [&](uint32_t p) {
-    const uint32_t at = 16u * p < last16 ? 16u * p : last16;
+    const uint32_t at = kb + 16u * p < last16 ? kb + 16u * p : last16;
 #pragma unroll
     for (int i = 0; i < kSRows; ++i) __builtin_memcpy(&sreg[i], sbase[i] + at, 16);
   };
   auto put_scales = [&](uint32_t p) {
-    const uint32_t d = 16u * p < last16 ? 0u : 16u * p - last16; // bytes, 15 at most if p is real
+    // bytes, 15 at most if there are such blocks
+    const uint32_t d = kb + 16u * p < last16 ? 0u : kb + 16u * p - last16;
     const uint32_t bits = 8u * (d & 7u);
 #pragma unroll
     for (int i = 0; i < kSRows; ++i) {
@@ -615,7 +627,8 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
       hi = d & 8u ? 0u : hi;
       lo = lo >> bits | (hi << 1) << (63u - bits);
       hi >>= bits;
-      *reinterpret_cast<u32x4_t *>(slds + (p & 1u) * kSBuf + (64u * NW * i + threadIdx.x) * 16u) =
+      if (WK > 1 && d > 15u) lo = hi = 0u; // a group may have none: no NaN in its zeros' place
+      *reinterpret_cast<u32x4_t *>(slds + (p & 1u) * kSBuf + (64u * NW * i + thread) * 16u) =
           (u32x4_t){(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     }
   };
@@ -766,6 +779,39 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *lds) {
   uint32_t tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
   const uint32_t l = tid & 63u, col32 = tid & 31u, half4 = (tid >> 5 & 1u) * 4u;
+  if constexpr (WK > 1) {
+    // the other groups' sums, added in their order; past what the waves write below
+    constexpr uint32_t kWave = MI * NI * 4096u, kAt = NW * 32u * (BM / WM * 4u + 16u);
+    static_assert(kAt + (WK - 1) * NW * kWave <= WK * kRegion, "the sums fit LDS");
+    uint8_t *const part = all_lds + kAt + wave * kWave + l * 16u;
+    if (group != 0u) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4_t *>(part + (group - 1u) * (NW * kWave) +
+                                         ((m * NI + n) * 4 + q) * 1024) =
+                (f32x4_t){acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2],
+                          acc[m][n][4 * q + 3]};
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (group != 0u) return;
+#pragma unroll
+    for (int g = 0; g < WK - 1; ++g)
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(
+                part + g * (NW * kWave) + ((m * NI + n) * 4 + q) * 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][n][4 * q + i] += v[i];
+          }
+  }
   constexpr int kStep = M == kGateUp ? 2 : 1, kBlocks = MI / kStep; // 32-row blocks of a wave
   const uint32_t wrow0 = row0 + wm * (kBlocks * 32u);               // the wave's first row of y
   if constexpr (kPacked) {
@@ -890,40 +936,41 @@ AXH_MX_TYPES(AXH_MX_KSPLIT_EXPERT, k32, 32, 8, 2)
 AXH_MX_TYPES(AXH_MX_KSPLIT_GATE_UP, k32, false, 4, 3)
 AXH_MX_KSPLIT_GATE_UP(mxfp4, TF32, k32, true, 4, 3)
 
-// Tile kernels: NAME, rows and columns of the tile, waves along both, buffers, waves
-// of a SIMD.
-#define AXH_MX_TILE_DENSE(TN, T, NAME, BM, BN, WM, WN, NBUF, WPE) \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN)      \
+// Tile kernels: NAME, rows and columns of the tile, waves along both and groups of
+// them along K, buffers of a group, waves of a SIMD.
+#define AXH_MX_TILE_DENSE(TN, T, NAME, BM, BN, WM, WN, WK, NBUF, WPE) \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK)      \
       __attribute__((amdgpu_waves_per_eu(WPE, WPE)))              \
       axh_mxfp4_matmul_##NAME##_##TN(AXH_MX_DENSE_ARGS) {         \
     extern __shared__ __align__(16) uint8_t tile[];               \
     AXH_MX_DENSE_UNPACK;                                          \
-    tile_body<kDense, T, false, BM, BN, WM, WN, NBUF>(a, tile);   \
+    tile_body<kDense, T, false, BM, BN, WM, WN, WK, NBUF>(a, tile);   \
   }
-#define AXH_MX_TILE_EXPERT(TN, T, NAME, BM, BN, WM, WN, NBUF, WPE) \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN)       \
+#define AXH_MX_TILE_EXPERT(TN, T, NAME, BM, BN, WM, WN, WK, NBUF, WPE) \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK)       \
       __attribute__((amdgpu_waves_per_eu(WPE, WPE)))               \
       axh_mxfp4_expert_matmul_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {  \
     extern __shared__ __align__(16) uint8_t tile[];                \
     AXH_MX_EXPERT_UNPACK;                                          \
-    tile_body<kGrouped, T, false, BM, BN, WM, WN, NBUF>(a, tile);  \
+    tile_body<kGrouped, T, false, BM, BN, WM, WN, WK, NBUF>(a, tile);  \
   }
-#define AXH_MX_TILE_GATE_UP(TN, T, NAME, PACKED, BM, BN, WM, WN, NBUF, WPE) \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN)                \
+#define AXH_MX_TILE_GATE_UP(TN, T, NAME, PACKED, BM, BN, WM, WN, WK, NBUF, WPE) \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK)                \
       __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                        \
       axh_mxfp4_expert_gate_up_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {          \
     extern __shared__ __align__(16) uint8_t tile[];                         \
     AXH_MX_EXPERT_UNPACK;                                                   \
-    tile_body<kGateUp, T, PACKED, BM, BN, WM, WN, NBUF>(a, tile);           \
+    tile_body<kGateUp, T, PACKED, BM, BN, WM, WN, WK, NBUF>(a, tile);           \
   }
 #define AXH_MX_TILE_EXPERTS(NAME, ...)                        \
   AXH_MX_TYPES(AXH_MX_TILE_EXPERT, NAME, __VA_ARGS__)         \
   AXH_MX_TYPES(AXH_MX_TILE_GATE_UP, NAME, false, __VA_ARGS__) \
   AXH_MX_TILE_GATE_UP(mxfp4, TF32, NAME, true, __VA_ARGS__)
-AXH_MX_TYPES(AXH_MX_TILE_DENSE, t64x64, 64, 64, 1, 2, 3, 1)
-AXH_MX_TYPES(AXH_MX_TILE_DENSE, t64x128, 64, 128, 1, 4, 3, 2)
-AXH_MX_TYPES(AXH_MX_TILE_DENSE, t128x128, 128, 128, 2, 2, 2, 2)
-AXH_MX_TYPES(AXH_MX_TILE_DENSE, t256x256, 256, 256, 2, 4, 2, 2)
-AXH_MX_TILE_EXPERTS(t128x64, 128, 64, 2, 2, 3, 2)
-AXH_MX_TILE_EXPERTS(t128x128, 128, 128, 2, 2, 2, 2)
-AXH_MX_TILE_EXPERTS(t256x256, 256, 256, 2, 4, 2, 2)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t64x64, 64, 64, 1, 2, 1, 3, 1)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t64x64s2, 64, 64, 1, 2, 2, 3, 1)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t64x128, 64, 128, 1, 4, 1, 3, 2)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t128x128, 128, 128, 2, 2, 1, 2, 2)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t256x256, 256, 256, 2, 4, 1, 2, 2)
+AXH_MX_TILE_EXPERTS(t128x64, 128, 64, 2, 2, 1, 3, 2)
+AXH_MX_TILE_EXPERTS(t128x128, 128, 128, 2, 2, 1, 2, 2)
+AXH_MX_TILE_EXPERTS(t256x256, 256, 256, 2, 4, 1, 2, 2)

@@ -116,32 +116,33 @@ constexpr MatmulKind k128x128 = {"t128x128", 128, 128, 256, 73728};
 constexpr MatmulKind k128x64 = {"t128x64", 128, 64, 256, 81920};
 constexpr MatmulKind k64x128 = {"t64x128", 64, 128, 256, 81920};
 constexpr MatmulKind k64x64 = {"t64x64", 64, 64, 128, 53248};
+constexpr MatmulKind k64x64s2 = {"t64x64s2", 64, 64, 256, 106496};
 constexpr MatmulKind kSplit32 = {"k32", 32, 32, 512, 131072};
 constexpr MatmulKind kSplit32GateUp = {"k32", 64, 32, 256, 147456};
 constexpr MatmulKind kSplit16 = {"k16", 16, 32, 512, 147456};
 constexpr uint32_t kTileMinBlocks = 16; // the tiles read 16 scales of a row at once
 
 // The largest tile that gives most of the 256 CUs one (and is not mostly empty): a
-// larger one reads less, but what has no tile waits.  14336 x 4096, us: 512
-// columns 128x128 31.9, 256x256 (112 tiles) 34.3, 64x64 51.8; 1024 columns 45.2 with
-// 256x256, 58.6 with 128x128; 256 columns 128x128 20.9, 64x128 22.6; 96 columns 64x128
-// 13.5, 128x128 18.9.  Where even 64x64 gives too few, the K-split kernel, if its own
-// tiles fit one round of workgroups (4096 x 4096, 64 columns: 6.6 against 8.7; 96
-// columns, 384 tiles: 64x64 9.2, K-split 11.7) or K is long (4096 x 14336, 128 columns:
-// 26.9 against 28.7), and in the latter case with half the rows if those fit too
-// (4096 x 14336, 32 columns: 14.0 against 16.3; 8192 x 8192, 64 columns: 64x64 18.6,
-// K-split 20.4).
+// larger one reads less, but what has no tile waits.  14336 x 4096, us: 1024 columns
+// 256x256 45.2, 128x128 58.6; 512 columns 34.3 (112 tiles), 31.9; 256 columns 128x128
+// 20.9, 64x128 22.3, 64x64 28.3.  64x128 where 64x64 would give more than one round:
+// 5001 x 5408, 256 columns, 15.5 against 17.8; 8192 x 8192, 128 columns (128 tiles), 21.6
+// against 16.1.  A round of 64x64 has its K axis shared by two groups of waves, more
+// rounds not: 14336 x 4096, 32 columns, 10.2 against 11.2; 28672 x 8192, 32 columns, 32.0
+// against 30.0.  The K-split kernel where its tiles are one round too: 4096 x 4096, 64
+// columns, 6.6 against 7.1; 128 columns (512 tiles) 12.3 against 7.7; with half the rows
+// if K is long and those fit as well: 4096 x 14336, 32 columns, 13.9 against 16.3; 4096 x
+// 4096 7.6 against 6.6.
 const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
   auto grid = [&](const MatmulKind &k) {
     return (uint64_t)div_up(n_rows, k.rows) * div_up(batch, k.cols);
   };
   if (nblk < kTileMinBlocks) return kSplit32;
-  for (const MatmulKind *k : {&k256x256, &k128x128, &k64x128})
-    if (grid(*k) >= 200u && batch > k->cols / 2u) return *k;
-  if (grid(k64x64) >= 200u) return k64x64;
-  const bool is_long = nblk >= 320u;
-  if (grid(kSplit32) > 256u && !is_long) return k64x64;
-  return is_long && grid(kSplit16) <= 256u ? kSplit16 : kSplit32;
+  if (batch > 128u && grid(k256x256) >= 200u) return k256x256;
+  if (batch > 64u && grid(k128x128) >= 200u) return k128x128;
+  if (batch > 64u && grid(k64x64) > 256u) return k64x128;
+  if (grid(kSplit32) <= 256u) return nblk >= 320u && grid(kSplit16) <= 256u ? kSplit16 : kSplit32;
+  return grid(k64x64) <= 256u ? k64x64s2 : k64x64;
 }
 
 // By the mean number of columns of an expert: tiles of 64 columns while most experts

@@ -243,7 +243,8 @@ def test_matvec_special_scales(ctx, dev):
 
 MATMULS = [(1, 32, 1), (3, 64, 2), (31, 224, 5), (33, 256, 32), (64, 288, 33), (100, 1312, 17),
            (129, 512, 64), (65, 544, 65), (128, 1024, 128), (300, 1056, 130), (1000, 96, 300),
-           (257, 4096, 77), (2048, 2048, 16), (1025, 736, 513)]
+           (257, 4096, 77), (2048, 2048, 16), (1025, 736, 513), (40, 10272, 20), (16500, 544, 33),
+           (2100, 512, 130), (2100, 1600, 520), (1700, 544, 1800), (3900, 512, 3300)]
 
 
 @pytest.mark.parametrize("t", [F32, F16, BF16])
@@ -292,15 +293,18 @@ def test_matmul_of_many_tiles_is_that_of_few(ctx, dev, axc):
     assert len(names) >= 3
 
 
-def test_matmul_special_scales(ctx, dev):
+@pytest.mark.parametrize("rows,cols,batches", [(70, 1056, (66, 20, 160)), (1100, 544, (300,)),
+                                               (2100, 512, (130,)), (700, 1600, (500,)),
+                                               (16500, 544, (33,))])
+def test_matmul_special_scales(ctx, dev, axc, rows, cols, batches):
     """A NaN block reaches its row (or column) only; blocks past a row's end are
     not multiplied with the next row's."""
-    rows, cols, batch = 70, 1056, 66
-    for b in (batch, 20, 160):
+    for b in batches:
+        _say(f"{rows}x{cols}x{b}: {axc.mxfp4_matmul_kernel_name(rows, cols, b)}")
         wc, ws = MX.gen_weights(1, rows, cols)
         xc, xs = MX.quantize(activations(b, b, cols))
         ws[11, 0] = 255
-        xs[9, 32] = 255
+        xs[9, -1] = 255
         dy = dev.out(rows * b * 4)
         ctx.mxfp4_matmul(dev.up(wc), dev.up(ws), dev.up(xc), dev.up(xs), dy, rows, cols, b)
         ctx.synchronize()

@@ -18,8 +18,8 @@ import pytest
 
 OBJDUMP = shutil.which("llvm-objdump") or "/opt/rocm/llvm/bin/llvm-objdump"
 # tile -> loads of a wave and step, of them of A, and buffers
-TILES = {"t64x64": (8, 4, 3), "t64x128": (6, 2, 3), "t128x64": (6, 4, 3), "t128x128": (8, 4, 2),
-         "t256x256": (8, 4, 2)}
+TILES = {"t64x64": (8, 4, 3), "t64x64s2": (8, 4, 3), "t64x128": (6, 2, 3), "t128x64": (6, 4, 3),
+         "t128x128": (8, 4, 2), "t256x256": (8, 4, 2)}
 
 
 @pytest.fixture(scope="module")
@@ -64,7 +64,7 @@ def _in_flight(body, extra=None):
 def _named(kernels, tile):
     named = [n for n in kernels if f"_{tile}_" in n]
     # dense products: 3 types; expert layers: 3, gate/up: 4
-    assert len(named) == {"t64x64": 3, "t64x128": 3, "t128x64": 7}.get(tile, 10)
+    assert len(named) == {"t64x64": 3, "t64x64s2": 3, "t64x128": 3, "t128x64": 7}.get(tile, 10)
     return named
 
 
