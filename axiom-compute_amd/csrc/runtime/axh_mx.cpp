@@ -245,13 +245,14 @@ axh_status axh_mxfp4_quantize(axh_context *ctx, uint32_t x_type, const void *x, 
   if (!aligned(codes, 16)) return bad("codes must be 16-byte aligned");
   const uint64_t blocks = (uint64_t)rows * (cols / 32u);
   if (blocks >= (1ull << 30)) return bad("too many blocks for one call");
-  // rows that follow one another are one long row
-  const bool flat = stride == cols;
-  const uint32_t words[] = {(uint32_t)blocks, flat ? (uint32_t)blocks : cols / 32u,
-                            (uint32_t)stride, (uint32_t)(stride >> 32)};
+  // Four loads of a lane at once where there are enough, of 16 bits: 8192 x 4096 15.3 us
+  // against 17.2, 2048 x 4096 5.0 against 4.7; f32 8192 x 4096 27.2 against 25.1.
+  const uint32_t per = size == 2u && blocks >= 1u << 19 ? 4u : 1u;
+  const uint32_t words[] = {(uint32_t)blocks, stride == cols ? 0u : cols / 32u, (uint32_t)stride,
+                            (uint32_t)(stride >> 32), per};
   void *bufs[] = {mut(x), codes, scales};
-  return launch(ctx, kElem, std::string("axh_mxfp4_quantize_") + type, div_up(blocks, 64u), 1, 256,
-                0, bufs, 3, words, 4, stream);
+  return launch(ctx, kElem, std::string("axh_mxfp4_quantize_") + type, div_up(blocks, 64u * per), 1,
+                256, 0, bufs, 3, words, 5, stream);
 }
 
 axh_status axh_mxfp4_dequant(axh_context *ctx, const void *codes, const void *scales,

@@ -158,7 +158,8 @@ def test_quantize_edge_blocks_bit_exact(ctx, dev, t):
 
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 @pytest.mark.parametrize("rows,cols,stride", [(1, 32, 0), (1, 4096, 0), (7, 96, 0), (5, 1312, 0),
-                                              (3, 416, 424), (65, 64, 1000), (257, 2048, 0)])
+                                              (3, 416, 424), (65, 64, 1000), (257, 2048, 0),
+                                              (4099, 4128, 4136)])
 def test_quantize_rows_and_strides(ctx, dev, t, rows, cols, stride):
     _say(f"quantize {rows}x{cols} stride {stride} type {t}")
     step = stride or cols
