@@ -95,9 +95,21 @@ template <> __device__ __forceinline__ void unpack2<TBF16>(uint32_t w, float &a,
   b = __builtin_bit_cast(float, w & 0xFFFF0000u);
 }
 
-// silu(g) * u with silu(g) = g / (1 + exp(-g)); exp(-g) overflows to infinity
-// below g = -88.7, where the quotient is -0 as it should be.
-__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u with silu(g) = g / (1 + 2^(-g log2 e)).  The exponent's rounding is
+// made good by a factor (a relative error of |g| / 2^24 else), and with the 1 ulp of
+// the exponential and of the reciprocal the result is within 5 ulp: the library's
+// exponential and an exact division cost three times the instructions, which in the
+// expert layers' epilogue counts (4096 tokens, 4 of 32 experts, 2048 x 1024: 80.6 us for
+// gate and up with those, 71.0 with these).  Past +-104 the exponential is 0 or infinite
+// in f32 whatever g is, and the reciprocal of infinity 0.
+__device__ __forceinline__ float swiglu(float g, float u) {
+  constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0cp-26f; // their sum: log2 e
+  const float n = __builtin_amdgcn_fmed3f(-g, -104.0f, 104.0f);
+  const float t = n * kLog2e;
+  const float rest = __builtin_fmaf(n, kRest, __builtin_fmaf(n, kLog2e, -t));
+  const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(rest, 0x1.62e43p-1f, 1.0f); // ln 2
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
 
 template <int kCtrl> __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, false);
