@@ -149,16 +149,17 @@ const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
 // have one of them, of 256 where an expert's outputs are many, so that such tiles are
 // mostly full and still many.  Gate and up / down, us.  40 experts, 1312 x 736, mean 50:
 // 128x64 15.7 / 10.4, 128x128 18.8 / 12.4.  64 experts, 2048 x 1408: mean 32: 46.5 / 27.1,
-// 55.9 / 29.5; mean 64: 58.7 / 38.1, 57.5 / 33.3; mean 256: 128x128 114 / 71, 256x256 134 /
-// 78; mean 512: 190 / 117, 189 / 107; mean 1024: 340 / 251, 332 / 219.  8 experts, 4096 x
-// 14336: mean 75: 124 / 65, 167 / 97; mean 175: 234 / 89, 186 / 104; mean 256: 322 / 159,
-// 269 / 121.
+// 55.9 / 29.5; mean 64: 58.7 / 38.1, 57.5 / 33.3.  128x128 and 256x256: 64 experts, 2048 x
+// 1408, mean 256: down 70.3, 63.0; mean 512: 188 / 115, 165 / 105; 32 experts, 2048 x
+// 1024, mean 256: 47.8 / 32.5, 53 / 33.2; mean 512: 77 / 49.5, 71 / 48; 2880 x 2880, mean
+// 256: 190 / 90, 167 / 95; 8 experts, 4096 x 14336, mean 75: 124 / 65, 167 / 97; mean 175:
+// 234 / 89, 174 / 92.
 const MatmulKind &expert_kind(uint32_t n_rows, uint32_t nblk, uint64_t slots, uint32_t n_experts,
                               bool gate_up) {
   const uint64_t mean = slots / n_experts;
   if (nblk < kTileMinBlocks) return gate_up ? kSplit32GateUp : kSplit32;
   if (mean <= 52u) return k128x64;
-  return mean >= 160u && mean * n_rows >= 1u << 20 ? k256x256 : k128x128;
+  return mean >= 160u && mean * n_rows >= 1u << 19 ? k256x256 : k128x128;
 }
 
 // Shared checks of the expert products for prompts.

@@ -513,7 +513,8 @@ def test_expert_layer_for_few_tokens(ctx, dev, tokens, top_k, n, hidden, ffn):
 
 
 PROMPTS = [(1, 1, 1, 64, 32), (7, 2, 5, 288, 64), (40, 4, 8, 512, 256), (333, 6, 40, 416, 96),
-           (300, 4, 4, 1312, 160), (700, 3, 8, 544, 288), (260, 1, 1, 256, 64)]
+           (300, 4, 4, 1312, 160), (700, 3, 8, 544, 288), (260, 1, 1, 256, 64),
+           (333, 6, 40, 544, 544), (300, 2, 130, 544, 576), (2100, 1, 2, 544, 1056)]
 
 
 @pytest.mark.parametrize("t", [F32, F16, BF16, MXFP4])
