@@ -635,21 +635,27 @@ def test_combine_odd_columns(ctx, dev, cols, t):
 
 
 def test_calls_on_another_stream_and_in_a_graph(ctx, dev, axc):
-    """One MXFP4 linear layer recorded in a graph gives, replay after replay
-    with eager work between, the eager result."""
+    """One MXFP4 linear layer on another stream, and recorded in a graph, replay
+    after replay with eager work between, gives the eager result."""
     rows, cols, batch = 160, 544, 40
     wc, ws = MX.gen_weights(1, rows, cols)
     x = activations(2, batch, cols)
     dx, dwc, dws = dev.up(x), dev.up(wc), dev.up(ws)
     dc, ds, dy = dev.out(batch * cols // 2), dev.out(batch * cols // 32), dev.out(rows * batch * 4)
 
-    def step():
-        ctx.mxfp4_quantize(dx, dc, ds, batch, cols)
-        ctx.mxfp4_matmul(dwc, dws, dc, ds, dy, rows, cols, batch)
+    def step(stream=None):
+        ctx.mxfp4_quantize(dx, dc, ds, batch, cols, stream=stream)
+        ctx.mxfp4_matmul(dwc, dws, dc, ds, dy, rows, cols, batch, stream=stream)
 
     step()
     ctx.synchronize()
     eager = dev.down(dy, rows * batch * 4, np.float32, (batch, rows))
+    other = axc.HipContext.new()
+    ctx.upload(dy, np.zeros(rows * batch * 4, dtype=np.uint8))
+    step(other.stream)
+    ctx.synchronize(other.stream)
+    assert np.array_equal(dev.down(dy, rows * batch * 4, np.float32, (batch, rows)), eager)
+    other.close()
     g = ctx.capture(step)
     assert g.node_count == 2
     for _ in range(3):
@@ -660,6 +666,102 @@ def test_calls_on_another_stream_and_in_a_graph(ctx, dev, axc):
         step()
         ctx.synchronize()
     g.close()
+
+
+# ---- an expert layer from a file -----------------------------------------------------------
+def _layer_file(axc, path, n, hidden, ffn, bias):
+    """Writes the layer blk.3 and returns its matrices, in 64 bits."""
+    gg, out, tensors = axc.gguf, {}, []
+    for i, (name, rows, cols) in enumerate((("ffn_gate_inp", (n,), hidden),
+                                            ("ffn_gate_exps", (n, ffn), hidden),
+                                            ("ffn_up_exps", (n, ffn), hidden),
+                                            ("ffn_down_exps", (n, hidden), ffn))):
+        c, s = MX.gen_weights(20 + i, *rows, cols)
+        out[name] = MX.decode(c, s)
+        tensors.append((f"blk.3.{name}.weight", MXFP4, (cols,) + rows[::-1],
+                        MX.to_ggml(c, s).tobytes()))
+    if bias is not None:
+        tensors.append(("blk.3.exp_probs_b.bias", F32, (n,), bias.tobytes()))
+    gg.write_gguf(path, [], tensors)
+    return out
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 4, 5, 70])
+def test_expert_layer_from_a_file(ctx, dev, axc, tmp_path, tokens):
+    """Each step of a layer's run against the formulas on the step before it, and
+    three replays of it in a graph."""
+    n, k, hidden, ffn = 12, 3, 544, 576
+    _say(f"expert layer, {tokens} tokens")
+    bias = np.linspace(-0.2, 0.2, n, dtype=np.float32)
+    w = _layer_file(axc, tmp_path / "layer.gguf", n, hidden, ffn, bias)
+    options = axc.RouteOptions(n_experts=n, top_k=k, score="sigmoid")
+    with axc.gguf.GgufFile(tmp_path / "layer.gguf") as f:
+        layer = axc.experts.ExpertLayer(ctx, f, "blk.3", options, max_tokens=70)
+    x = activations(30, tokens, hidden)
+    dx, dy = dev.up(x), dev.out(tokens * hidden * 4)
+    layer.run(dx, dy, tokens)
+    ctx.synchronize()
+    y = dev.down(dy, tokens * hidden * 4, np.float32, (tokens, hidden))
+
+    def get(buf, dtype, shape):
+        nbytes = int(np.prod(shape)) * np.dtype(dtype).itemsize
+        return np.frombuffer(ctx.download(buf, nbytes), dtype=dtype).reshape(shape)
+
+    few = tokens <= layer.few_tokens
+    xq = MX.decode(*MX.quantize(x))
+    xr = x.astype(np.float64) if tokens == 1 else xq
+    logits = get(layer.logits, np.float32, (tokens, n)).astype(np.float64)
+    bound = hidden * U23 * (np.abs(xr) @ np.abs(w["ffn_gate_inp"]).T)
+    assert (np.abs(logits - xr @ w["ffn_gate_inp"].T) <= bound).all()
+    e, wt = MX.route(logits, k, "sigmoid", bias=bias)
+    assert np.array_equal(get(layer.experts, np.int32, (tokens, k)), e)
+    got = get(layer.weights, np.float32, (tokens, k)).astype(np.float64)
+    assert (np.abs(got - wt) <= 64 * U23 * np.abs(wt)).all()
+    if few:
+        h = get(layer.h, np.float32, (tokens, k, ffn)).astype(np.float64)
+    else:
+        h = MX.decode(get(layer.h_codes, np.uint8, (tokens, k, ffn // 2)),
+                      get(layer.h_scales, np.uint8, (tokens, k, ffn // 32)))
+    for t in range(tokens):
+        want, bound = np.zeros(hidden), np.zeros(hidden)
+        for i in range(k):
+            xt = x[t].astype(np.float64) if few else xq[t]
+            wg, wu = w["ffn_gate_exps"][e[t, i]], w["ffn_up_exps"][e[t, i]]
+            exact = MX.swiglu(wg @ xt, wu @ xt)
+            ulp = _swiglu_bound(wg @ xt, wu @ xt, *(hidden * U23 * (np.abs(m) @ np.abs(xt))
+                                                    for m in (wg, wu)))
+            # MXFP4: half a step, or what is cut off above 6, is at most a quarter of the
+            # block's largest magnitude
+            step = 0 if few else np.repeat(np.abs(exact).reshape(-1, 32).max(axis=1) / 4, 32)
+            assert (np.abs(h[t, i] - exact) <= ulp + step).all()
+            wd = w["ffn_down_exps"][e[t, i]]
+            want += got[t, i] * (wd @ h[t, i])
+            bound += (2 * ffn + k + 1) * U24 * got[t, i] * (np.abs(wd) @ np.abs(h[t, i]))
+        assert (np.abs(y[t] - want) <= bound).all()
+    g = ctx.capture(lambda: layer.run(dx, dy, tokens))
+    for _ in range(3):
+        ctx.upload(dy, np.zeros(tokens * hidden * 4, dtype=np.uint8))
+        g.launch()
+        ctx.synchronize()
+        assert np.array_equal(dev.down(dy, tokens * hidden * 4, np.float32, y.shape), y)
+        layer.run(dx, dy, tokens)
+        ctx.synchronize()
+    g.close()
+    layer.close()
+
+
+def test_expert_layer_refusals(ctx, axc, tmp_path):
+    _layer_file(axc, tmp_path / "layer.gguf", 4, 64, 32, np.zeros(4, dtype=np.float32))
+    with axc.gguf.GgufFile(tmp_path / "layer.gguf") as f:
+        make = axc.experts.ExpertLayer
+        for prefix, n, t in (("blk.4", 4, 8), ("blk.3", 5, 8), ("blk.3", 4, 0)):
+            with pytest.raises(ValueError):
+                make(ctx, f, prefix, axc.RouteOptions(n_experts=n, top_k=1), max_tokens=t)
+        layer = make(ctx, f, "blk.3", axc.RouteOptions(n_experts=4, top_k=1), max_tokens=8)
+    with pytest.raises(ValueError):
+        layer.run(layer.slots, layer.slots, 9)
+    layer.run(layer.slots, layer.slots, 0)
+    layer.close()
 
 
 # ---- refusals ------------------------------------------------------------------------------
