@@ -47,21 +47,21 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax) {
   return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
 }
 
-// 2^(127 - e), the exact factor that brings a block of scale byte e (0 .. 252,
-// what mx_scale_byte gives for finite blocks) to E2M1's range; 0 for 255, whose
-// codes are zeros.
-__device__ __forceinline__ float mx_inverse(uint32_t e) {
-  return __builtin_bit_cast(float, e == 255u ? 0u : (254u - e) << 23);
+// The divisor of the converting instructions for a block of scale byte e (0 .. 252,
+// what mx_scale_byte gives for finite blocks): they read its exponent field only, so
+// 0 stands for 2^-127.
+__device__ __forceinline__ float mx_divisor(uint32_t e) {
+  return __builtin_bit_cast(float, e << 23);
 }
 
-// Eight values, already multiplied by mx_inverse, as eight codes: round to
-// nearest even, magnitudes above 6 become 6 (v_cvt_scalef32_pk_fp4_f32).
-__device__ __forceinline__ uint32_t fp4_pack8(const float *v) {
+// Eight values of a block with that divisor as eight codes: round to nearest even,
+// magnitudes above 6 become 6 (v_cvt_scalef32_pk_fp4_f32).
+__device__ __forceinline__ uint32_t fp4_pack8(const float *v, float divisor) {
   uint32_t c = 0;
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], 1.0f, 0);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], 1.0f, 1);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], 1.0f, 2);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], 1.0f, 3);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], divisor, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], divisor, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], divisor, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], divisor, 3);
   return c;
 }
 

@@ -51,10 +51,9 @@ template <> __device__ __forceinline__ void store8<TBF16>(uint8_t *p, const floa
 // Quantisation.  Four lanes share a block of 32 elements, eight each (one or
 // two 16-byte loads): the block's largest magnitude is a maximum over bit
 // patterns (magnitudes order like integers, NaN above infinity), two DPP steps
-// inside the quad.  The conversion divides by the block's power of two, which is
-// exact, so each element is rounded once: f32 multiplied by its inverse, f16 and
-// bf16 two at a time by the converting instruction itself, as the instructions, not
-// the bytes, would else bound the kernel.  8192 x 4096 bf16: 15.3 us (20.3 through f32
+// inside the quad.  The converting instruction divides by the block's power of two,
+// which is exact, so each element is rounded once; f16 and bf16 go through it as they
+// are, as the instructions, not the bytes, would else bound the kernel.  8192 x 4096 bf16: 15.3 us (20.3 through f32
 // and with a division a block), 5.5 TB/s.
 // ---------------------------------------------------------------------------
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
@@ -80,7 +79,7 @@ template <class T> struct Eight { // elements of 16 bits
     return __builtin_bit_cast(uint32_t, lo);
   }
   __device__ __forceinline__ uint32_t codes(uint32_t e) const {
-    const float scale = __builtin_bit_cast(float, e << 23);
+    const float scale = mx_divisor(e);
     uint32_t c = 0;
     if constexpr (__is_same(T, TF16)) {
       c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, pair<half2_t>(0), scale, 0);
@@ -116,11 +115,7 @@ template <> struct Eight<TF32> {
     return o > m ? o : m;
   }
   __device__ __forceinline__ uint32_t codes(uint32_t e) const {
-    const float f = mx_inverse(e);
-    float u[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = v[i] * f;
-    return fp4_pack8(u);
+    return fp4_pack8(v, mx_divisor(e));
   }
 };
 
@@ -167,7 +162,8 @@ __device__ __forceinline__ void quantize_body(const uint8_t *x, uint8_t *codes, 
 }
 
 // ---------------------------------------------------------------------------
-// Decoding: eight codes (one dword) a lane.
+// Decoding: eight codes (one dword) a lane, 32 bytes (16) of f32 (f16, bf16) out: bound
+// by the stores.  8192 x 4096 to bf16: 13.3 us, 6.4 TB/s.
 // ---------------------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ void dequant_body(const uint8_t *codes, const uint8_t *scales,
@@ -232,6 +228,9 @@ extern "C" __global__ void __launch_bounds__(256) axh_mxfp4_unpack_ggml(const ui
 // cannot be chosen, so a round of the top-k is a maximum over the wave (DPP),
 // and the lowest expert among equals is the first set bit of the first
 // non-empty ballot.
+//   Bound by latency for few tokens (1.7 us for one of 32 experts), by the vector
+// instructions for many: 4096 x 256 experts, 8 chosen from 4 of 8 groups, 8.3 us, about a
+// thousand of them a token (its bytes would take 0.9).
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -550,7 +549,8 @@ extern "C" __global__ void __launch_bounds__(1024) axh_expert_plan(const int32_t
 // y[t] = sum over a token's choices of weight * slot output, in f32, rounded
 // once.  Choices outside 0 .. n_experts - 1 (the router's -1 among them) are left
 // out: their slots hold nothing.  Eight columns a lane where n_cols is a multiple of
-// eight and the rows are 16-byte aligned, else one.
+// eight and the rows are 16-byte aligned, else one.  Bound by memory: 4096 tokens of 4
+// choices, 2048 columns, bf16, 13.3 us, 6.3 TB/s.
 // ---------------------------------------------------------------------------
 namespace {
 

@@ -10,6 +10,11 @@
 // consecutive blocks (1 KiB of codes) of 64 / LPR rows.  The waves of a group
 // have a unit each and the same rows; a group's partial sums meet in LDS, in
 // the units' order.
+//   128256 x 4096: 46.7 us, 6.0 TB/s.  4096 x 14336 (31 MB, 6.0 us at the rate of a
+// copy): 8.5 us in a loop, of which a launch and the wait for the activations and the
+// first codes are about 3.  8 choices of 64 experts, 2048 x 1024: gate and up 6.9 us (3.4
+// for the bytes), down 5.9 (1.7); two batches of loads a wave, so that what bounds
+// them is the chain of launch, expert, codes and sum.
 #include "mx_common.h"
 
 using namespace axh;
