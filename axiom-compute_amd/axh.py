@@ -16,6 +16,7 @@ this module fails loudly when it has not been built; there is no fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass, field
 from pathlib import Path
@@ -464,6 +465,7 @@ class RouteOptions:
     normalize: bool = True
     scale: float = 1.0
 
+    @functools.cached_property
     def _c(self) -> _RouteOptions:
         if self.score not in SCORES:
             raise ValueError(f"unknown score {self.score!r}")
@@ -973,7 +975,7 @@ class HipContext:
                      logits_type: int = GGML_F32, stream=None) -> None:
         """experts (int32), weights (f32): n_tokens x top_k choices from router logits;
         bias: f32 per expert or None."""
-        o = options._c()
+        o = options._c
         _check(self._lib.axh_expert_route(self._raw, logits_type, _ptr(logits), _ptr(bias),
                                           _ptr(experts), _ptr(weights), n_tokens, ctypes.byref(o),
                                           _stream(stream)))
