@@ -229,8 +229,8 @@ extern "C" __global__ void __launch_bounds__(256) axh_mxfp4_unpack_ggml(const ui
 // and the lowest expert among equals is the first set bit of the first
 // non-empty ballot.
 //   Bound by latency for few tokens (1.7 us for one of 32 experts), by the vector
-// instructions for many: 4096 x 256 experts, 8 chosen from 4 of 8 groups, 8.3 us, about a
-// thousand of them a token (its bytes would take 0.9).
+// instructions for many: 4096 x 256 experts, 8 chosen from 4 of 8 groups, 7.8 us, about
+// 650 of them a token (its bytes would take 0.9).
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -297,7 +297,7 @@ __device__ __forceinline__ void route_body(const uint8_t *logits, const float *b
                                            uint32_t group_best, float scale, uint32_t *lds) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t token = blockIdx.x * 4u + wave;
-  const bool real = token < n_tokens; // waves past the end only keep barriers company
+  const bool real = token < n_tokens;
   const uint8_t *row = logits + (uint64_t)(real ? token : 0u) * n_experts * T::kBytes;
   const float kInf = __builtin_inff();
 
@@ -339,10 +339,10 @@ __device__ __forceinline__ void route_body(const uint8_t *logits, const float *b
   if (n_groups > 1u) {
     // Every lane looks at its part of one group: 64 / G lanes (a power of two)
     // per group, then the two best of the lanes of a group are merged.
-    uint32_t *mine = lds + wave * (64u * NPL + 64u);
+    uint32_t *mine = lds + wave * (64u * NPL);
 #pragma unroll
     for (int j = 0; j < NPL; ++j) mine[64u * j + lane] = key[j];
-    __syncthreads();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the wave's own
     const uint32_t per = n_experts / n_groups;
     uint32_t log_lanes = 0;
     while ((n_groups << (log_lanes + 1u)) <= 64u) ++log_lanes;
@@ -365,20 +365,21 @@ __device__ __forceinline__ void route_body(const uint8_t *logits, const float *b
     uint32_t gk = a;
     if (group_best == 2u)
       gk = order_of((a ? value_of(a) : -kInf) + (b ? value_of(b) : -kInf));
-    uint32_t *gkeys = mine + 64u * NPL;
-    if (g < n_groups && part == 0u) gkeys[g] = gk;
-    __syncthreads();
-    uint32_t rank = 0; // of group `lane`: greater ones and equal ones before it
-    const uint32_t own = lane < n_groups ? gkeys[lane] : 0u;
+    // lane g: group g's key, and its rank: greater ones and equal ones before it
+    const uint32_t at0 = (uint32_t)__shfl((int)gk, (int)(lane << log_lanes & 63u));
+    const uint32_t own = lane < n_groups ? at0 : 0u;
+    uint32_t rank = 0;
     for (uint32_t i = 0; i < n_groups; ++i) {
-      const uint32_t k = gkeys[i];
+      const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)own, (int)i);
       rank += k > own || (k == own && i < lane) ? 1u : 0u;
     }
     const uint64_t kept = __ballot(lane < n_groups && rank < groups_kept);
+    // e / per by a product, exact for e and per up to 1024
+    const uint32_t inverse = (1u << 20) / per + 1u;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
       const uint32_t e = 64u * j + lane;
-      if (e < n_experts && !((kept >> (e / per)) & 1u)) key[j] = 0u;
+      if (e < n_experts && !((kept >> (e * inverse >> 20)) & 1u)) key[j] = 0u;
     }
   }
 
@@ -424,7 +425,7 @@ __device__ __forceinline__ void route_body(const uint8_t *logits, const float *b
       const uint8_t *logits, const float *bias, int32_t *experts, float *weights,                 \
       uint32_t n_tokens, uint32_t n_experts, uint32_t top_k, uint32_t flags, uint32_t n_groups,   \
       uint32_t groups_kept, uint32_t group_best, uint32_t scale) {                                \
-    __shared__ uint32_t lds[4 * (64 * NPL + 64)];                                                 \
+    __shared__ uint32_t lds[4 * 64 * NPL];                                                 \
     route_body<T, NPL>(logits, bias, experts, weights, n_tokens, n_experts, top_k, flags,         \
                        n_groups, groups_kept, group_best, __builtin_bit_cast(float, scale), lds); \
   }
