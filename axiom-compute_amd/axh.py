@@ -264,6 +264,7 @@ def load_library(path: Optional[Path] = None) -> ctypes.CDLL:
         "axh_mxfp4_matvec": (st, [vp, vp, vp, vp, vp, u32, u32, vp]),
         "axh_mxfp4_matmul": (st, [vp, vp, vp, vp, vp, u32, vp, u32, u32, u32, vp]),
         "axh_mxfp4_matmul_kernel_name": (st, [u32, u32, u32, u32, c.c_char_p, sz]),
+        "axh_expert_logits": (st, [vp, u32, vp, vp, vp, u32, u32, u32, vp]),
         "axh_expert_route": (st, [vp, u32, vp, vp, vp, vp, u32, c.POINTER(_RouteOptions), vp]),
         "axh_mxfp4_expert_gate_up": (st, [vp, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32,
                                           vp]),
@@ -970,6 +971,12 @@ class HipContext:
         _check(self._lib.axh_mxfp4_matmul(self._raw, _ptr(w_codes), _ptr(w_scales), _ptr(x_codes),
                                           _ptr(x_scales), y_type, _ptr(y), n_rows, cols, batch,
                                           _stream(stream)))
+
+    def expert_logits(self, w, x, logits, n_experts: int, cols: int, n_tokens: int,
+                      w_type: int = GGML_F32, stream=None) -> None:
+        """logits (n_tokens x n_experts) = the router's product W x, all in f32."""
+        _check(self._lib.axh_expert_logits(self._raw, w_type, _ptr(w), _ptr(x), _ptr(logits),
+                                           n_experts, cols, n_tokens, _stream(stream)))
 
     def expert_route(self, logits, bias, experts, weights, n_tokens: int, options: RouteOptions,
                      logits_type: int = GGML_F32, stream=None) -> None:

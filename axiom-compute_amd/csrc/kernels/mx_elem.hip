@@ -440,6 +440,155 @@ AXH_ROUTE_N(8)
 AXH_ROUTE_N(16)
 
 // ---------------------------------------------------------------------------
+// Router logits: logits[t][e] = sum over k of W[e][k] * x[t][k], f32 x, W of f32, f16 or
+// bf16 (exact in f32), products and sums in f32, so that the choice of the experts does
+// not depend on a quantisation.
+//   Few tokens: a wave an expert and token, eight elements a lane and step, four steps
+// requested at once.
+//   More: v_mfma_f32_32x32x2_f32 over tiles of kT * 32 tokens by kT * 32 experts, K shared
+// among the waves in chunks of 32 elements and joined through LDS in the waves' order.
+// The two halves of a wave hold the two halves of a chunk, sixteen elements a lane, so a
+// row's chunk is a whole 128-byte line and operands need no LDS: an instruction's k
+// indexes are elements j and 16 + j of the chunk in both operands.  The next chunk is
+// requested before the products of this one.  Tiles of the same tokens run on one XCD.
+// ---------------------------------------------------------------------------
+namespace {
+
+template <class T>
+__device__ __forceinline__ void logits_row_body(const float *x, const uint8_t *w, float *logits,
+                                                uint32_t n_tokens, uint32_t n_experts,
+                                                uint32_t cols) {
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t e = blockIdx.x * 4u + (threadIdx.x >> 6), t = blockIdx.y;
+  if (e >= n_experts || t >= n_tokens) return;
+  const uint8_t *xr = reinterpret_cast<const uint8_t *>(x + (uint64_t)t * cols);
+  const uint8_t *wr = w + (uint64_t)e * cols * T::kBytes;
+  const uint32_t pieces = cols / 8u;
+  float acc[4] = {};
+  uint32_t p = 0;
+  for (; p + 256u <= pieces; p += 256u) {
+    float a[4][8], b[4][8];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      load8<T>(wr + (uint64_t)(p + 64u * i + lane) * 8u * T::kBytes, a[i]);
+      load8<TF32>(xr + (uint64_t)(p + 64u * i + lane) * 32u, b[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i] = __builtin_fmaf(a[i][j], b[i][j], acc[i]);
+  }
+  for (p += lane; p < pieces; p += 64u) {
+    float a[8], b[8];
+    load8<T>(wr + (uint64_t)p * 8u * T::kBytes, a);
+    load8<TF32>(xr + (uint64_t)p * 32u, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j & 3] = __builtin_fmaf(a[j], b[j], acc[j & 3]);
+  }
+  const float sum = wave_sum_f32((acc[0] + acc[1]) + (acc[2] + acc[3]));
+  if (lane == 0u) logits[(uint64_t)t * n_experts + e] = sum;
+}
+
+// Sixteen elements of each of kT rows, 32 apart.
+template <class T, int kT> struct Sixteen {
+  float v[kT][16];
+  __device__ __forceinline__ void load(const uint8_t *const (&rows)[kT], uint32_t k) {
+#pragma unroll
+    for (int i = 0; i < kT; ++i) {
+      load8<T>(rows[i] + (uint64_t)k * T::kBytes, v[i]);
+      load8<T>(rows[i] + (uint64_t)(k + 8u) * T::kBytes, v[i] + 8);
+    }
+  }
+};
+
+template <class T, int kT, int kWaves>
+__device__ __forceinline__ void logits_tile_body(const float *x, const uint8_t *w, float *logits,
+                                                 uint32_t n_tokens, uint32_t n_experts,
+                                                 uint32_t cols, uint32_t tiles, float *lds) {
+  constexpr uint32_t kSide = 32u * kT, kOuts = kSide * kSide;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t tile = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (tile >= tiles) return; // the whole workgroup
+  const uint32_t across = (n_experts + kSide - 1u) / kSide;
+  const uint32_t t0 = tile / across * kSide, e0 = tile % across * kSide;
+  const uint32_t r = lane & 31u, half = lane >> 5;
+  // rows past the last are the last one's: their outputs are not stored
+  const uint8_t *xr[kT], *wr[kT];
+#pragma unroll
+  for (int i = 0; i < kT; ++i) {
+    const uint32_t t = t0 + 32u * i + r, e = e0 + 32u * i + r;
+    xr[i] = reinterpret_cast<const uint8_t *>(x) +
+            (uint64_t)(t < n_tokens ? t : n_tokens - 1u) * cols * 4u;
+    wr[i] = w + (uint64_t)(e < n_experts ? e : n_experts - 1u) * cols * T::kBytes;
+  }
+  f32x16_t acc[kT][kT] = {};
+  const uint32_t chunks = cols / 32u;
+  if (wave < chunks) {
+    Sixteen<TF32, kT> a, an;
+    Sixteen<T, kT> b, bn;
+    a.load(xr, wave * 32u + half * 16u);
+    b.load(wr, wave * 32u + half * 16u);
+    for (uint32_t c = wave; c < chunks; c += kWaves) {
+      const uint32_t next = c + kWaves < chunks ? c + kWaves : c;
+      an.load(xr, next * 32u + half * 16u);
+      bn.load(wr, next * 32u + half * 16u);
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int m = 0; m < kT; ++m)
+#pragma unroll
+          for (int n = 0; n < kT; ++n)
+            acc[m][n] =
+                __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[m][j], b.v[n][j], acc[m][n], 0, 0, 0);
+      a = an;
+      b = bn;
+    }
+  }
+  // output v of a lane: token 8 * (v / 4) + 4 * half + v % 4, expert r of its 32 x 32
+#pragma unroll
+  for (int m = 0; m < kT; ++m)
+#pragma unroll
+    for (int n = 0; n < kT; ++n)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        lds[wave * kOuts + ((m * kT + n) * 16 + v) * 64u + lane] = acc[m][n][v];
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < kOuts; i += 64u * kWaves) {
+    float sum = lds[i];
+#pragma unroll
+    for (uint32_t k = 1; k < kWaves; ++k) sum += lds[k * kOuts + i];
+    const uint32_t v = i >> 6 & 15u, mn = i >> 10; // lane is i & 63 here too
+    const uint32_t t = t0 + mn / kT * 32u + (v >> 2) * 8u + half * 4u + (v & 3u);
+    const uint32_t e = e0 + mn % kT * 32u + r;
+    if (t < n_tokens && e < n_experts) logits[(uint64_t)t * n_experts + e] = sum;
+  }
+}
+
+} // namespace
+
+#define AXH_LOGITS(NAME, T)                                                                       \
+  extern "C" __global__ void __launch_bounds__(256) axh_expert_logits_row_##NAME(                 \
+      const float *x, const uint8_t *w, float *logits, uint32_t n_tokens, uint32_t n_experts,     \
+      uint32_t cols, uint32_t) {                                                                  \
+    logits_row_body<T>(x, w, logits, n_tokens, n_experts, cols);                                  \
+  }                                                                                               \
+  extern "C" __global__ void __launch_bounds__(1024) axh_expert_logits_t32_##NAME(                \
+      const float *x, const uint8_t *w, float *logits, uint32_t n_tokens, uint32_t n_experts,     \
+      uint32_t cols, uint32_t tiles) {                                                            \
+    extern __shared__ float sums[];                                                               \
+    logits_tile_body<T, 1, 16>(x, w, logits, n_tokens, n_experts, cols, tiles, sums);             \
+  }                                                                                               \
+  extern "C" __global__ void __launch_bounds__(512) axh_expert_logits_t64_##NAME(                 \
+      const float *x, const uint8_t *w, float *logits, uint32_t n_tokens, uint32_t n_experts,     \
+      uint32_t cols, uint32_t tiles) {                                                            \
+    extern __shared__ float sums[];                                                               \
+    logits_tile_body<T, 2, 8>(x, w, logits, n_tokens, n_experts, cols, tiles, sums);              \
+  }
+AXH_LOGITS(f32, TF32)
+AXH_LOGITS(f16, TF16)
+AXH_LOGITS(bf16, TBF16)
+
+// ---------------------------------------------------------------------------
 // The order of slots by expert: a stable counting sort.  Slot i is choice
 // i % top_k of token i / top_k.  A workgroup gives a contiguous chunk of the
 // slots their places, a wave of it a contiguous part of the chunk; it counts the

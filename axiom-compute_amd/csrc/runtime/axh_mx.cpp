@@ -162,6 +162,8 @@ const MatmulKind &expert_kind(uint32_t n_rows, uint32_t nblk, uint64_t slots, ui
   return mean >= 160u && mean * n_rows >= 1u << 19 ? k256x256 : k128x128;
 }
 
+constexpr uint32_t kFewLogits = 8, kLogitTiles = 200;
+
 // Shared checks of the expert products for prompts.
 axh_status check_experts(axh_context *ctx, uint32_t n_rows, uint32_t cols, uint32_t n_tokens,
                          uint32_t top_k, uint32_t n_experts) {
@@ -332,6 +334,36 @@ axh_status axh_mxfp4_matmul(axh_context *ctx, const void *w_codes, const void *w
   return launch(ctx, kMatmul, std::string("axh_mxfp4_matmul_") + k.name + "_" + type,
                 (uint64_t)row_tiles * div_up(batch, k.cols), 1, k.threads, k.lds, bufs, 5, words, 4,
                 stream);
+}
+
+axh_status axh_expert_logits(axh_context *ctx, uint32_t w_type, const void *w, const float *x,
+                             float *logits, uint32_t n_experts, uint32_t cols, uint32_t n_tokens,
+                             void *stream) {
+  if (!ctx) return bad("ctx is NULL");
+  const char *type = type_name(w_type);
+  if (!type) return bad("w_type must be f32, f16 or bf16");
+  axh_status s = check_cols(cols);
+  if (s != AXH_OK) return s;
+  if (n_experts == 0 || n_experts > kMaxExperts) return bad("n_experts must be 1 to 1024");
+  if (n_tokens >= kMaxBuffer) return bad("too many tokens");
+  if (n_tokens == 0) return ok();
+  if (!w || !x || !logits) return bad("NULL device pointer");
+  if (!aligned(w, 16) || !aligned(x, 16) || !aligned(logits, 4))
+    return bad("w and x must be 16-byte and logits 4-byte aligned");
+  void *bufs[] = {const_cast<float *>(x), mut(w), logits};
+  const std::string name = "axh_expert_logits_";
+  if (n_tokens <= kFewLogits) {
+    const uint32_t words[] = {n_tokens, n_experts, cols, 0};
+    return launch(ctx, kElem, name + "row_" + type, div_up(n_experts, 4u), n_tokens, 256, 0, bufs,
+                  3, words, 4, stream);
+  }
+  const uint64_t large = (uint64_t)div_up(n_tokens, 64u) * div_up(n_experts, 64u);
+  const bool t64 = n_experts > 32u && large >= kLogitTiles;
+  const uint64_t tiles =
+      t64 ? large : (uint64_t)div_up(n_tokens, 32u) * div_up(n_experts, 32u);
+  const uint32_t words[] = {n_tokens, n_experts, cols, (uint32_t)tiles};
+  return launch(ctx, kElem, name + (t64 ? "t64_" : "t32_") + type, 8u * div_up(tiles, 8u), 1,
+                t64 ? 512 : 1024, t64 ? 131072 : 65536, bufs, 3, words, 4, stream);
 }
 
 axh_status axh_expert_route(axh_context *ctx, uint32_t logits_type, const void *logits,

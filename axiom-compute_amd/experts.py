@@ -9,8 +9,9 @@ gate and up products with SiLU, their down products, and the weighted sum.
 
 Tensors are those of a GGUF layer `prefix`: ffn_gate_exps.weight and
 ffn_up_exps.weight (hidden x ffn x experts, ne[0] first), ffn_down_exps.weight (ffn x
-hidden x experts) and ffn_gate_inp.weight (hidden x experts), of type MXFP4; and
-exp_probs_b.bias (experts, f32) where the router adds a bias to its choices.
+hidden x experts), of type MXFP4; the router's ffn_gate_inp.weight (hidden x experts), f32,
+f16 or bf16 (its product is in f32 then), or MXFP4; and exp_probs_b.bias (experts, f32)
+where the router adds a bias to its choices.
 
 The codes and scales are laid out once, when the layer is made, and so are the
 workspaces: run() allocates nothing and can be captured in a graph.  No counterpart
@@ -46,6 +47,23 @@ class _Matrix:
         self.scales.close()
 
 
+class _Router:
+    """The router's matrix: f32, f16 or bf16 as it stands in the file, or MXFP4."""
+
+    def __init__(self, ctx, file: GgufFile, name: str):
+        t = file.tensors[name]
+        self.type, self.packed = t.type, None
+        if t.type == GGML_MXFP4:
+            self.packed = _Matrix(ctx, file, name)
+        elif t.type in (_axh.GGML_F32, _axh.GGML_F16, _axh.GGML_BF16):
+            self.w = file.upload(ctx, name)
+        else:
+            raise ValueError(f"{name} is of type {t.type}, not MXFP4, f32, f16 or bf16")
+
+    def close(self) -> None:
+        (self.packed or self.w).close()
+
+
 class ExpertLayer:
     """Up to few_tokens tokens, run() takes the single-token products, which read the
     weights of each choice and keep the activations in f32; more tokens are
@@ -76,8 +94,9 @@ class ExpertLayer:
             raise ValueError(f"the tensors' shapes do not make a layer of {options.n_experts} "
                              f"experts: {shapes}")
         self.hidden, self.ffn = hidden, ffn
-        self.router, self.gate, self.up, self.down = (
-            _Matrix(ctx, file, names[k]) for k in ("ffn_gate_inp", "ffn_gate_exps", "ffn_up_exps",
+        self.router = _Router(ctx, file, names["ffn_gate_inp"])
+        self.gate, self.up, self.down = (
+            _Matrix(ctx, file, names[k]) for k in ("ffn_gate_exps", "ffn_up_exps",
                                                    "ffn_down_exps"))
         bias = f"{prefix}.exp_probs_b.bias"
         self.bias = None
@@ -103,14 +122,18 @@ class ExpertLayer:
         ctx, n, k = self.ctx, self.options.n_experts, self.options.top_k
         hidden, ffn = self.hidden, self.ffn
         few = n_tokens <= self.few_tokens
-        if n_tokens != 1 or not few:
+        router = self.router.packed
+        if not few or (router and n_tokens != 1):
             ctx.mxfp4_quantize(x, self.x_codes, self.x_scales, n_tokens, hidden, GGML_F32,
                                stream=stream)
-        if n_tokens == 1 and few:
-            ctx.mxfp4_matvec(self.router.codes, self.router.scales, x, self.logits, n, hidden,
+        if not router:
+            ctx.expert_logits(self.router.w, x, self.logits, n, hidden, n_tokens,
+                              self.router.type, stream=stream)
+        elif n_tokens == 1 and few:
+            ctx.mxfp4_matvec(router.codes, router.scales, x, self.logits, n, hidden,
                              stream=stream)
         else:
-            ctx.mxfp4_matmul(self.router.codes, self.router.scales, self.x_codes, self.x_scales,
+            ctx.mxfp4_matmul(router.codes, router.scales, self.x_codes, self.x_scales,
                              self.logits, n, hidden, n_tokens, stream=stream)
         ctx.expert_route(self.logits, self.bias, self.experts, self.weights, n_tokens,
                          self.options, stream=stream)

@@ -331,6 +331,65 @@ def test_matmul_one_hot_is_exact(ctx, dev):
 
 
 # ---- routing -------------------------------------------------------------------------
+# experts, cols, tokens: one kernel for up to 8 tokens, tiles of 32 x 32, and of 64 x 64 from
+# 200 of them (the last two)
+LOGITS = [(1, 32, 1), (5, 96, 3), (64, 4096, 1), (7, 2080, 8), (256, 2048, 2), (1, 32, 9),
+          (33, 544, 9), (32, 2048, 70), (128, 1312, 77), (1000, 96, 40), (257, 512, 2500),
+          (1024, 288, 830)]
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("n,cols,tokens", LOGITS)
+def test_expert_logits(ctx, dev, n, cols, tokens, t):
+    _say(f"logits {n} x {cols}, {tokens} tokens, type {t}")
+    rng = np.random.default_rng(n + cols)
+    raw, w = as_type(rng.standard_normal((n, cols)).astype(np.float32) / 8, t)
+    x = activations(41, tokens, cols)
+    dw, dx, dy = dev.up(raw), dev.up(x), dev.out(tokens * n * 4)
+    ctx.expert_logits(dw, dx, dy, n, cols, tokens, t)
+    ctx.synchronize()
+    y = dev.down(dy, tokens * n * 4, np.float32, (tokens, n)).astype(np.float64)
+    x = x.astype(np.float64)
+    w = w.astype(np.float64)
+    assert (np.abs(y - x @ w.T) <= (cols + 1) * U23 * (np.abs(x) @ np.abs(w).T)).all()
+    # a row with a single 1 takes one element, and a token's NaN stays its own
+    k = (np.arange(n) * 37 + 5) % cols
+    one = np.zeros((n, cols), dtype=np.float32)
+    one[np.arange(n), k] = 1
+    xs = activations(42, tokens, cols)
+    dw, dx = dev.up(as_type(one, t)[0]), dev.up(xs)
+    ctx.expert_logits(dw, dx, dy, n, cols, tokens, t)
+    ctx.synchronize()
+    y = dev.down(dy, tokens * n * 4, np.float32, (tokens, n))
+    assert np.array_equal(y, xs[:, k])
+    xs[tokens // 2, cols // 2] = np.nan
+    dx = dev.up(xs)
+    ctx.expert_logits(dw, dx, dy, n, cols, tokens, t)
+    ctx.synchronize()
+    nan = np.isnan(dev.down(dy, tokens * n * 4, np.float32, (tokens, n)))
+    assert nan[tokens // 2].all() and nan.sum() == n
+
+
+def test_expert_logits_refusals(ctx, dev, axc):
+    p = dev.out(1 << 12)
+    good = dict(w=p, x=p, y=p, n=4, cols=64, tokens=2, t=F32)
+
+    def call(**k):
+        a = good | k
+        ctx.expert_logits(a["w"], a["x"], a["y"], a["n"], a["cols"], a["tokens"], a["t"])
+
+    for k in (dict(w=None), dict(x=None), dict(y=None), dict(w=p + 8), dict(x=p + 4),
+              dict(y=p + 2), dict(n=0), dict(n=1025), dict(cols=0), dict(cols=48),
+              dict(cols=1 << 23), dict(tokens=1 << 31), dict(t=MXFP4), dict(t=2)):
+        with pytest.raises(axc.DispatchError) as err:
+            call(**k)
+            pytest.fail(f"{k} was accepted")
+        assert err.value.variant == "InvalidArgument", k
+    call(tokens=0)
+    ctx.synchronize()
+    assert (dev.down(p, 1 << 12, np.uint8, (1 << 12,)) == 0xA5).all()
+
+
 def _route(ctx, dev, axc, logits, bias=None, t=F32, **kw):
     tokens, n = logits.shape
     raw, values = as_type(logits, t)
@@ -747,6 +806,65 @@ def test_expert_layer_from_a_file(ctx, dev, axc, tmp_path, tokens):
         layer.run(dx, dy, tokens)
         ctx.synchronize()
     g.close()
+    layer.close()
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens", [1, 3, 70])
+def test_expert_layer_with_a_router_of_floats(ctx, dev, axc, tmp_path, tokens, t):
+    """The layer is the calls one after another, with the router's product in f32."""
+    n, k, hidden, ffn = 12, 3, 544, 576
+    _say(f"expert layer, router of type {t}, {tokens} tokens")
+    path = tmp_path / "layer.gguf"
+    _layer_file(axc, path, n, hidden, ffn, None)
+    rng = np.random.default_rng(50)
+    raw, w = as_type(rng.standard_normal((n, hidden)).astype(np.float32) / 16, t)
+    with axc.gguf.GgufFile(path) as f:
+        rest = [(name, s.type, tuple(s.shape), f.tensor_bytes(name))
+                for name, s in f.tensors.items() if "gate_inp" not in name]
+    axc.gguf.write_gguf(path, [], [("blk.3.ffn_gate_inp.weight", t, (hidden, n),
+                                    raw.tobytes())] + rest)
+    options = axc.RouteOptions(n_experts=n, top_k=k)
+    with axc.gguf.GgufFile(path) as f:
+        layer = axc.experts.ExpertLayer(ctx, f, "blk.3", options, max_tokens=70, few_tokens=4)
+    x = activations(51, tokens, hidden)
+    dx, dy = dev.up(x), dev.out(tokens * hidden * 4)
+    layer.run(dx, dy, tokens)
+    ctx.synchronize()
+    y = dev.down(dy, tokens * hidden * 4, np.float32, (tokens, hidden))
+    logits = np.frombuffer(ctx.download(layer.logits, tokens * n * 4), dtype=np.float32)
+    logits = logits.reshape(tokens, n).astype(np.float64)
+    x64, w64 = x.astype(np.float64), w.astype(np.float64)
+    assert (np.abs(logits - x64 @ w64.T)
+            <= (hidden + 1) * U23 * (np.abs(x64) @ np.abs(w64).T)).all()
+    chosen = np.frombuffer(ctx.download(layer.experts, tokens * k * 4), dtype=np.int32)
+    assert np.array_equal(chosen.reshape(tokens, k), MX.route(logits, k)[0])
+    again = dev.out(tokens * hidden * 4)
+    g, u, d = layer.gate, layer.up, layer.down
+    if tokens <= 4:
+        ctx.mxfp4_expert_gate_up(g.codes, g.scales, u.codes, u.scales, dx, layer.experts, layer.h,
+                                 ffn, hidden, tokens, k, n)
+        ctx.mxfp4_expert_down(d.codes, d.scales, layer.h, layer.experts, layer.weights, again,
+                              hidden, ffn, tokens, k, n)
+    else:
+        ctx.mxfp4_quantize(dx, layer.x_codes, layer.x_scales, tokens, hidden)
+        ctx.expert_plan(layer.experts, layer.plan, tokens, k, n)
+        ctx.mxfp4_expert_gate_up_matmul(g.codes, g.scales, u.codes, u.scales, layer.x_codes,
+                                        layer.x_scales, layer.plan, layer.h_codes, layer.h_scales,
+                                        ffn, hidden, tokens, k, n)
+        ctx.mxfp4_expert_matmul(d.codes, d.scales, layer.h_codes, layer.h_scales, layer.plan,
+                                layer.slots, hidden, ffn, tokens, k, n)
+        ctx.expert_combine(layer.slots, layer.experts, layer.weights, again, hidden, tokens, k,
+                           n_experts=n)
+    ctx.synchronize()
+    assert np.array_equal(dev.down(again, tokens * hidden * 4, np.float32, y.shape), y)
+    graph = ctx.capture(lambda: layer.run(dx, dy, tokens))
+    for _ in range(3):
+        ctx.upload(dy, np.zeros(tokens * hidden * 4, dtype=np.uint8))
+        graph.launch()
+        ctx.synchronize()
+        assert np.array_equal(dev.down(dy, tokens * hidden * 4, np.float32, y.shape), y)
+    graph.close()
     layer.close()
 
 
