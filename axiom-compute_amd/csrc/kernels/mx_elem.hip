@@ -443,14 +443,17 @@ AXH_ROUTE_N(16)
 // Router logits: logits[t][e] = sum over k of W[e][k] * x[t][k], f32 x, W of f32, f16 or
 // bf16 (exact in f32), products and sums in f32, so that the choice of the experts does
 // not depend on a quantisation.
-//   Few tokens: a wave an expert and token, eight elements a lane and step, four steps
-// requested at once.
-//   More: v_mfma_f32_32x32x2_f32 over tiles of kT * 32 tokens by kT * 32 experts, K shared
-// among the waves in chunks of 32 elements and joined through LDS in the waves' order.
-// The two halves of a wave hold the two halves of a chunk, sixteen elements a lane, so a
-// row's chunk is a whole 128-byte line and operands need no LDS: an instruction's k
-// indexes are elements j and 16 + j of the chunk in both operands.  The next chunk is
-// requested before the products of this one.  Tiles of the same tokens run on one XCD.
+//   Few logits: a wave each, eight elements a lane and step, four steps requested at once.
+// 256 x 7168, one token, 3.9 us in a loop of calls (a launch).
+//   More: v_mfma_f32_16x16x4_f32 over tiles of 16, 32 or 64 tokens by as many experts, K
+// shared among the waves in chunks of 32 elements and joined through LDS in the waves'
+// order.  A wave brings its chunk to LDS of its own by whole 128-byte lines, as f32, and
+// has no one to wait for; the next chunk is on its way during the products.  (Fragments
+// loaded straight from memory, a line for each lane, were bound by the cache's lookups: 256
+// x 4096, 4096 tokens, 108 us.)  An instruction's k indexes are elements 8 g + j of the
+// chunk, g the lane's quarter, in both operands.  Tiles of the same tokens run on one XCD.
+//   Bound by the matrix units: 4096 tokens, 256 x 4096 80 us, 256 x 7168 136 us, 107 and
+// 111 TFLOP/s.  For fewer tokens, the 16 waves of few workgroups: 100 tokens 9.3 and 14.7.
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -489,14 +492,38 @@ __device__ __forceinline__ void logits_row_body(const float *x, const uint8_t *w
   if (lane == 0u) logits[(uint64_t)t * n_experts + e] = sum;
 }
 
-// Sixteen elements of each of kT rows, 32 apart.
-template <class T, int kT> struct Sixteen {
-  float v[kT][16];
-  __device__ __forceinline__ void load(const uint8_t *const (&rows)[kT], uint32_t k) {
+// A chunk of a wave's kRows rows, 32 elements of each, on its way to LDS: 16-byte loads of
+// consecutive lanes along a row.
+template <class T, int kRows> struct Chunk {
+  static constexpr uint32_t kPer = 16u / T::kBytes;  // elements of a load
+  static constexpr uint32_t kAcross = 32u / kPer, kStep = 64u / kAcross; // loads a row, rows a step
+  u32x4_t v[kRows / kStep];
+  __device__ __forceinline__ void load(const uint8_t *base, uint32_t first, uint32_t n,
+                                       uint32_t cols, uint32_t k, uint32_t lane) {
 #pragma unroll
-    for (int i = 0; i < kT; ++i) {
-      load8<T>(rows[i] + (uint64_t)k * T::kBytes, v[i]);
-      load8<T>(rows[i] + (uint64_t)(k + 8u) * T::kBytes, v[i] + 8);
+    for (uint32_t i = 0; i < kRows / kStep; ++i) {
+      // rows past the last are the last one's: their outputs are not stored
+      const uint32_t r = first + kStep * i + lane / kAcross;
+      v[i] = *reinterpret_cast<const u32x4_t *>(
+          base + ((uint64_t)(r < n ? r : n - 1u) * cols + k + lane % kAcross * kPer) * T::kBytes);
+    }
+  }
+  // As f32 rows of 128 bytes; 16-byte piece q of row r is at q ^ (r / 2 % 8), so that the
+  // sixteen rows of a read meet all banks.
+  __device__ __forceinline__ void store(float *lds, uint32_t lane) const {
+#pragma unroll
+    for (uint32_t i = 0; i < kRows / kStep; ++i) {
+      const uint32_t r = kStep * i + lane / kAcross, q = lane % kAcross, x = r >> 1 & 7u;
+      f32x4_t *row = reinterpret_cast<f32x4_t *>(lds + r * 32u);
+      if constexpr (T::kBytes == 4u) {
+        row[q ^ x] = __builtin_bit_cast(f32x4_t, v[i]);
+      } else {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) unpack2<T>(v[i][j], f[2 * j], f[2 * j + 1]);
+        row[(2u * q) ^ x] = (f32x4_t){f[0], f[1], f[2], f[3]};
+        row[(2u * q + 1u) ^ x] = (f32x4_t){f[4], f[5], f[6], f[7]};
+      }
     }
   }
 };
@@ -505,85 +532,89 @@ template <class T, int kT, int kWaves>
 __device__ __forceinline__ void logits_tile_body(const float *x, const uint8_t *w, float *logits,
                                                  uint32_t n_tokens, uint32_t n_experts,
                                                  uint32_t cols, uint32_t tiles, float *lds) {
-  constexpr uint32_t kSide = 32u * kT, kOuts = kSide * kSide;
+  constexpr uint32_t kSide = 16u * kT, kOuts = kSide * kSide, kMine = 64u * kSide;
+  static_assert(kOuts <= kMine, "a wave's outputs take the place of its chunks");
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t tile = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   if (tile >= tiles) return; // the whole workgroup
   const uint32_t across = (n_experts + kSide - 1u) / kSide;
   const uint32_t t0 = tile / across * kSide, e0 = tile % across * kSide;
-  const uint32_t r = lane & 31u, half = lane >> 5;
-  // rows past the last are the last one's: their outputs are not stored
-  const uint8_t *xr[kT], *wr[kT];
-#pragma unroll
-  for (int i = 0; i < kT; ++i) {
-    const uint32_t t = t0 + 32u * i + r, e = e0 + 32u * i + r;
-    xr[i] = reinterpret_cast<const uint8_t *>(x) +
-            (uint64_t)(t < n_tokens ? t : n_tokens - 1u) * cols * 4u;
-    wr[i] = w + (uint64_t)(e < n_experts ? e : n_experts - 1u) * cols * T::kBytes;
-  }
-  f32x16_t acc[kT][kT] = {};
+  const uint32_t r = lane & 15u, quarter = lane >> 4, swizzle = r >> 1;
+  float *mine = lds + wave * kMine;
+  const uint8_t *xb = reinterpret_cast<const uint8_t *>(x);
+  f32x4_t acc[kT][kT] = {};
   const uint32_t chunks = cols / 32u;
   if (wave < chunks) {
-    Sixteen<TF32, kT> a, an;
-    Sixteen<T, kT> b, bn;
-    a.load(xr, wave * 32u + half * 16u);
-    b.load(wr, wave * 32u + half * 16u);
+    Chunk<TF32, kSide> a;
+    Chunk<T, kSide> b;
+    a.load(xb, t0, n_tokens, cols, wave * 32u, lane);
+    b.load(w, e0, n_experts, cols, wave * 32u, lane);
     for (uint32_t c = wave; c < chunks; c += kWaves) {
+      a.store(mine, lane);
+      b.store(mine + kSide * 32u, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the wave's own
       const uint32_t next = c + kWaves < chunks ? c + kWaves : c;
-      an.load(xr, next * 32u + half * 16u);
-      bn.load(wr, next * 32u + half * 16u);
+      a.load(xb, t0, n_tokens, cols, next * 32u, lane);
+      b.load(w, e0, n_experts, cols, next * 32u, lane);
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
+      for (uint32_t h = 0; h < 2; ++h) {
+        f32x4_t fa[kT], fb[kT];
+        const uint32_t at = ((2u * quarter + h) ^ swizzle) * 4u;
 #pragma unroll
-        for (int m = 0; m < kT; ++m)
+        for (int i = 0; i < kT; ++i) {
+          fa[i] = *reinterpret_cast<const f32x4_t *>(mine + (16u * i + r) * 32u + at);
+          fb[i] = *reinterpret_cast<const f32x4_t *>(mine + (kSide + 16u * i + r) * 32u + at);
+        }
 #pragma unroll
-          for (int n = 0; n < kT; ++n)
-            acc[m][n] =
-                __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[m][j], b.v[n][j], acc[m][n], 0, 0, 0);
-      a = an;
-      b = bn;
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int m = 0; m < kT; ++m)
+#pragma unroll
+            for (int n = 0; n < kT; ++n)
+              acc[m][n] =
+                  __builtin_amdgcn_mfma_f32_16x16x4f32(fa[m][j], fb[n][j], acc[m][n], 0, 0, 0);
+      }
+      asm volatile("" ::: "memory"); // the reads stay before the next chunk's stores
     }
   }
-  // output v of a lane: token 8 * (v / 4) + 4 * half + v % 4, expert r of its 32 x 32
+  // output v of a lane: token 4 * quarter + v, expert r of its 16 x 16
 #pragma unroll
   for (int m = 0; m < kT; ++m)
 #pragma unroll
     for (int n = 0; n < kT; ++n)
 #pragma unroll
-      for (int v = 0; v < 16; ++v)
-        lds[wave * kOuts + ((m * kT + n) * 16 + v) * 64u + lane] = acc[m][n][v];
+      for (int v = 0; v < 4; ++v)
+        mine[((m * kT + n) * 4 + v) * 64u + lane] = acc[m][n][v];
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < kOuts; i += 64u * kWaves) {
     float sum = lds[i];
 #pragma unroll
-    for (uint32_t k = 1; k < kWaves; ++k) sum += lds[k * kOuts + i];
-    const uint32_t v = i >> 6 & 15u, mn = i >> 10; // lane is i & 63 here too
-    const uint32_t t = t0 + mn / kT * 32u + (v >> 2) * 8u + half * 4u + (v & 3u);
-    const uint32_t e = e0 + mn % kT * 32u + r;
+    for (uint32_t k = 1; k < kWaves; ++k) sum += lds[k * kMine + i];
+    const uint32_t v = i >> 6 & 3u, mn = i >> 8; // lane is i & 63 here too
+    const uint32_t t = t0 + mn / kT * 16u + quarter * 4u + v;
+    const uint32_t e = e0 + mn % kT * 16u + r;
     if (t < n_tokens && e < n_experts) logits[(uint64_t)t * n_experts + e] = sum;
   }
 }
 
 } // namespace
 
+#define AXH_LOGITS_TILE(NAME, T, SIDE, WAVES)                                                     \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES) axh_expert_logits_t##SIDE##_##NAME(    \
+      const float *x, const uint8_t *w, float *logits, uint32_t n_tokens, uint32_t n_experts,     \
+      uint32_t cols, uint32_t tiles) {                                                            \
+    extern __shared__ float sums[];                                                               \
+    logits_tile_body<T, SIDE / 16, WAVES>(x, w, logits, n_tokens, n_experts, cols, tiles, sums);  \
+  }
 #define AXH_LOGITS(NAME, T)                                                                       \
   extern "C" __global__ void __launch_bounds__(256) axh_expert_logits_row_##NAME(                 \
       const float *x, const uint8_t *w, float *logits, uint32_t n_tokens, uint32_t n_experts,     \
-      uint32_t cols, uint32_t) {                                                                  \
+      uint32_t cols) {                                                                            \
     logits_row_body<T>(x, w, logits, n_tokens, n_experts, cols);                                  \
   }                                                                                               \
-  extern "C" __global__ void __launch_bounds__(1024) axh_expert_logits_t32_##NAME(                \
-      const float *x, const uint8_t *w, float *logits, uint32_t n_tokens, uint32_t n_experts,     \
-      uint32_t cols, uint32_t tiles) {                                                            \
-    extern __shared__ float sums[];                                                               \
-    logits_tile_body<T, 1, 16>(x, w, logits, n_tokens, n_experts, cols, tiles, sums);             \
-  }                                                                                               \
-  extern "C" __global__ void __launch_bounds__(512) axh_expert_logits_t64_##NAME(                 \
-      const float *x, const uint8_t *w, float *logits, uint32_t n_tokens, uint32_t n_experts,     \
-      uint32_t cols, uint32_t tiles) {                                                            \
-    extern __shared__ float sums[];                                                               \
-    logits_tile_body<T, 2, 8>(x, w, logits, n_tokens, n_experts, cols, tiles, sums);              \
-  }
+  AXH_LOGITS_TILE(NAME, T, 16, 16)                                                                \
+  AXH_LOGITS_TILE(NAME, T, 32, 16)                                                                \
+  AXH_LOGITS_TILE(NAME, T, 64, 8)
 AXH_LOGITS(f32, TF32)
 AXH_LOGITS(f16, TF16)
 AXH_LOGITS(bf16, TBF16)

@@ -162,7 +162,12 @@ const MatmulKind &expert_kind(uint32_t n_rows, uint32_t nblk, uint64_t slots, ui
   return mean >= 160u && mean * n_rows >= 1u << 19 ? k256x256 : k128x128;
 }
 
-constexpr uint32_t kFewLogits = 8, kLogitTiles = 200;
+// The router's product: a wave a logit up to 6144 logits (256 experts, 7168 columns, us: 16
+// tokens 9.3 against 13.6 with tiles of 16 x 16, 32 tokens 17.2 against 14.0; 4096 columns
+// 5.2 / 8.1 and 9.0 / 8.4), then the largest tile that most of the CUs get one of: 7168
+// columns, 333 tokens, 16 x 16 25.6 and 32 x 32 43.9 (88 tiles), 1024 tokens 54.9 / 48.2;
+// 2048 tokens, 32 x 32 86.9 and 64 x 64 126.7 (128 tiles), 4096 tokens 170.9 / 135.9.
+constexpr uint32_t kFewLogits = 6144, kLogitTiles = 200;
 
 // Shared checks of the expert products for prompts.
 axh_status check_experts(axh_context *ctx, uint32_t n_rows, uint32_t cols, uint32_t n_tokens,
@@ -352,18 +357,20 @@ axh_status axh_expert_logits(axh_context *ctx, uint32_t w_type, const void *w, c
     return bad("w and x must be 16-byte and logits 4-byte aligned");
   void *bufs[] = {const_cast<float *>(x), mut(w), logits};
   const std::string name = "axh_expert_logits_";
-  if (n_tokens <= kFewLogits) {
-    const uint32_t words[] = {n_tokens, n_experts, cols, 0};
+  if ((uint64_t)n_tokens * n_experts <= kFewLogits) {
+    const uint32_t words[] = {n_tokens, n_experts, cols};
     return launch(ctx, kElem, name + "row_" + type, div_up(n_experts, 4u), n_tokens, 256, 0, bufs,
-                  3, words, 4, stream);
+                  3, words, 3, stream);
   }
-  const uint64_t large = (uint64_t)div_up(n_tokens, 64u) * div_up(n_experts, 64u);
-  const bool t64 = n_experts > 32u && large >= kLogitTiles;
-  const uint64_t tiles =
-      t64 ? large : (uint64_t)div_up(n_tokens, 32u) * div_up(n_experts, 32u);
+  auto grid = [&](uint32_t side) {
+    return (uint64_t)div_up(n_tokens, side) * div_up(n_experts, side);
+  };
+  const uint32_t side = grid(64) >= kLogitTiles ? 64u : grid(32) >= kLogitTiles ? 32u : 16u;
+  const uint64_t tiles = grid(side);
   const uint32_t words[] = {n_tokens, n_experts, cols, (uint32_t)tiles};
-  return launch(ctx, kElem, name + (t64 ? "t64_" : "t32_") + type, 8u * div_up(tiles, 8u), 1,
-                t64 ? 512 : 1024, t64 ? 131072 : 65536, bufs, 3, words, 4, stream);
+  return launch(ctx, kElem, name + "t" + std::to_string(side) + "_" + type,
+                8u * div_up(tiles, 8u), 1, side == 64u ? 512 : 1024, side == 16u ? 65536 : 131072,
+                bufs, 3, words, 4, stream);
 }
 
 axh_status axh_expert_route(axh_context *ctx, uint32_t logits_type, const void *logits,

@@ -64,6 +64,7 @@ axh_status axh_mxfp4_matmul(axh_context *ctx, const void *w_codes, const void *w
 axh_status axh_mxfp4_matmul_kernel_name(uint32_t n_rows, uint32_t cols, uint32_t batch,
                                         uint32_t y_type, char *buf, size_t cap);
 
+/* ---- routing ---------------------------------------------------------------- */
 /* The router's product: logits[t * n_experts + e] = sum_k W[e][k] * x[t][k], W (n_experts x
  * cols) f32, f16 or bf16, x (n_tokens x cols) and logits f32, products and sums in f32 for
  * any number of tokens (their order depends on it).  w and x 16-byte aligned, cols a
@@ -71,9 +72,7 @@ axh_status axh_mxfp4_matmul_kernel_name(uint32_t n_rows, uint32_t cols, uint32_t
 axh_status axh_expert_logits(axh_context *ctx, uint32_t w_type, const void *w, const float *x,
                              float *logits, uint32_t n_experts, uint32_t cols, uint32_t n_tokens,
                              void *stream);
-
-/* ---- routing ----------------------------------------------------------------
- * Choices and weights of n_tokens tokens from their router logits (f32, f16 or
+/* Choices and weights of n_tokens tokens from their router logits (f32, f16 or
  * bf16, n_tokens x n_experts).  The score of an expert is the softmax over the
  * token's logits or the sigmoid of its logit; the order is by key, the score
  * plus the expert's bias (f32, NULL for none), the lowest expert first among

@@ -331,11 +331,12 @@ def test_matmul_one_hot_is_exact(ctx, dev):
 
 
 # ---- routing -------------------------------------------------------------------------
-# experts, cols, tokens: one kernel for up to 8 tokens, tiles of 32 x 32, and of 64 x 64 from
-# 200 of them (the last two)
+# experts, cols, tokens: a wave a logit for few, then tiles of 16 x 16, 64 x 64 (257 and
+# 1024 experts) and 32 x 32 (500)
 LOGITS = [(1, 32, 1), (5, 96, 3), (64, 4096, 1), (7, 2080, 8), (256, 2048, 2), (1, 32, 9),
           (33, 544, 9), (32, 2048, 70), (128, 1312, 77), (1000, 96, 40), (257, 512, 2500),
-          (1024, 288, 830)]
+          (1024, 288, 830), (500, 416, 401), (700, 32, 9),
+          (5, 2080, 1300)]
 
 
 @pytest.mark.parametrize("t", [F32, F16, BF16])

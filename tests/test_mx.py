@@ -163,6 +163,11 @@ def test_calls_without_a_context_are_refused(axc):
         assert status == 100
 
 
+def test_router_product_without_a_context_is_refused(axc):
+    lib = axc.load_library()
+    assert lib.axh_expert_logits(None, 0, None, None, None, 4, 32, 1, None) != 0
+
+
 def test_unknown_score_is_refused(axc):
     with pytest.raises(ValueError):
         axc.RouteOptions(n_experts=4, top_k=1, score="max")._c()
