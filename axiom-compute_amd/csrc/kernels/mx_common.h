@@ -101,7 +101,8 @@ template <> __device__ __forceinline__ void unpack2<TBF16>(uint32_t w, float &a,
 // exponential and an exact division cost three times the instructions, which in the
 // expert layers' epilogue counts (4096 tokens, 4 of 32 experts, 2048 x 1024: 80.6 us for
 // gate and up with those, 71.0 with these).  Past +-104 the exponential is 0 or infinite
-// in f32 whatever g is, and the reciprocal of infinity 0.
+// in f32 whatever g is, and the reciprocal of infinity 0.  Below g = -87.3 the reciprocal is
+// subnormal and may be 0, where silu(g) is less than 2e-36.
 __device__ __forceinline__ float swiglu(float g, float u) {
   constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0cp-26f; // their sum: log2 e
   const float n = __builtin_amdgcn_fmed3f(-g, -104.0f, 104.0f);

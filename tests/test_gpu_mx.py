@@ -810,6 +810,19 @@ def test_expert_layer_from_a_file(ctx, dev, axc, tmp_path, tokens):
     layer.close()
 
 
+def test_expert_layer_refuses_a_router_of_another_type(ctx, axc, tmp_path):
+    n, hidden, path = 4, 64, tmp_path / "layer.gguf"
+    _layer_file(axc, path, n, hidden, 32, None)
+    with axc.gguf.GgufFile(path) as f:
+        rest = [(name, s.type, tuple(s.shape), f.tensor_bytes(name))
+                for name, s in f.tensors.items() if "gate_inp" not in name]
+    axc.gguf.write_gguf(path, [], [("blk.3.ffn_gate_inp.weight", 2, (hidden, n),
+                                    bytes(n * hidden // 32 * 18))] + rest)
+    with axc.gguf.GgufFile(path) as f, pytest.raises(ValueError, match="is of type 2"):
+        axc.experts.ExpertLayer(ctx, f, "blk.3", axc.RouteOptions(n_experts=n, top_k=1),
+                                max_tokens=8)
+
+
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 @pytest.mark.parametrize("tokens", [1, 3, 70])
 def test_expert_layer_with_a_router_of_floats(ctx, dev, axc, tmp_path, tokens, t):
