@@ -501,13 +501,17 @@ __device__ __forceinline__ void ksplit_body(const Args &a, uint8_t *lds) {
 //   WK groups of such waves may share the K axis, each with buffers of its own, so
 // that twice the bytes are on their way where a CU has one workgroup; the groups'
 // sums meet in LDS.
+//   kShort: rows of fewer than 16 blocks, two steps at most.  A row's scales come with
+// the next rows' behind them, or, at the end of the array, with those before; they are
+// shifted down and the others cleared, as a NaN would pass through the codes' zeros.
 // ---------------------------------------------------------------------------
 template <Mode M, class T, bool kPacked, int BM, int BN, int WM, int WN, int WK,
-          int NBUF>
+          int NBUF, bool kShort = false>
 __device__ __forceinline__ void tile_body(const Args &a, uint8_t *all_lds) {
   constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
   constexpr int kSRows = (BM + BN + 64 * NW - 1) / (64 * NW); // rows of scales per lane
   constexpr uint32_t kBuf = (BM + BN) * 128u, kSBuf = kSRows * 64u * NW * 16u;
+  constexpr int kLate = kShort ? 0 : kSRows; // loads of scales behind those of a step
   constexpr int kLoads = (BM + BN) / 8 / NW; // per wave and step; rows of A first
   constexpr int kALoads = BM / 8 / NW, kHalf = kLoads / 2;
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads per wave");
@@ -610,12 +614,51 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *all_lds) {
   // further back, and shifted down by put_scales
   u32x4_t sreg[kSRows];
   const uint32_t last16 = nblk - 16u;
+  uint32_t back[kSRows]; // kShort: bytes from where the load begins to the row
+  if constexpr (kShort) {
+    const uint64_t all_a = (uint64_t)(M == kDense ? 1u : a.n_experts) * a.n_rows * nblk;
+    const uint64_t all_b = (uint64_t)a.n_x * nblk; // (both 16 at least)
+#pragma unroll
+    for (int i = 0; i < kSRows; ++i) {
+      const uint32_t r = 64u * NW * i + thread;
+      const bool is_a = r < (uint32_t)BM;
+      const bool up = is_a && M == kGateUp && ((r >> 5) & 1u);
+      const uint8_t *end = is_a ? (up ? a.us : a.ws) + all_a : a.xs + all_b;
+      const uint32_t rest = end - sbase[i] < 16 ? (uint32_t)(end - sbase[i]) : 16u;
+      back[i] = 16u - rest;
+      sbase[i] -= back[i];
+    }
+  }
   auto get_scales = [&](uint32_t p) {
+    if constexpr (kShort) { // one load in all: the waits count none behind it
+      if (p == 0u)
+#pragma unroll
+        for (int i = 0; i < kSRows; ++i) __builtin_memcpy(&sreg[i], sbase[i], 16);
+      return;
+    }
     const uint32_t at = kb + 16u * p < last16 ? kb + 16u * p : last16;
 #pragma unroll
     for (int i = 0; i < kSRows; ++i) __builtin_memcpy(&sreg[i], sbase[i] + at, 16);
   };
   auto put_scales = [&](uint32_t p) {
+    if constexpr (kShort) {
+      const uint64_t all = p ? 0ull : ~0ull; // steps past the row: zeros
+      const uint64_t in_lo = nblk >= 8u ? all : all & ((1ull << 8u * nblk) - 1u);
+      const uint64_t in_hi = nblk > 8u ? all & ((1ull << 8u * (nblk - 8u)) - 1u) : 0u;
+#pragma unroll
+      for (int i = 0; i < kSRows; ++i) {
+        const uint32_t shift = 8u * (back[i] & 7u);
+        uint64_t lo = (uint64_t)sreg[i].y << 32 | sreg[i].x;
+        uint64_t hi = (uint64_t)sreg[i].w << 32 | sreg[i].z;
+        lo = back[i] & 8u ? hi : lo;
+        hi = back[i] & 8u ? 0u : hi;
+        lo = (lo >> shift | (hi << 1) << (63u - shift)) & in_lo;
+        hi = hi >> shift & in_hi;
+        *reinterpret_cast<u32x4_t *>(slds + (p & 1u) * kSBuf + (64u * NW * i + thread) * 16u) =
+            (u32x4_t){(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+      }
+      return;
+    }
     // bytes, 15 at most if there are such blocks
     const uint32_t d = kb + 16u * p < last16 ? 0u : kb + 16u * p - last16;
     const uint32_t bits = 8u * (d & 7u);
@@ -724,7 +767,7 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *all_lds) {
     multiply(f0, c, k0);
     interleave(kSecond);
     __builtin_amdgcn_sched_barrier(0);
-    if (kOdd) get_scales((s >> 1) + 2u); // behind the requests above
+    if (kOdd && !kShort) get_scales((s >> 1) + 2u); // behind the requests above
     read_frags(f0, 2, buf);
     multiply(f1, c, k1);
     interleave(kNone);
@@ -736,7 +779,7 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *all_lds) {
     // step s + 1 has landed: of the younger loads, NBUF - 2 steps' and, in an odd step
     // or with a third buffer, the scales', may be on their way
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
-                     (NBUF - 2) * kLoads + (kOdd || NBUF > 2 ? kSRows : 0))
+                     (NBUF - 2) * kLoads + (kOdd || NBUF > 2 ? kLate : 0))
                  : "memory");
     __builtin_amdgcn_sched_barrier(0);
     loads(f0, 0, then, s + NBUF, buf, 0, kHalf);
@@ -753,9 +796,9 @@ __device__ __forceinline__ void tile_body(const Args &a, uint8_t *all_lds) {
 #pragma unroll
   for (int i = 0; i < kHalf; ++i) request(NBUF - 1u, NBUF - 1u, i);
   put_scales(0);
-  get_scales(1);
+  if (!kShort) get_scales(1);
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(
-                   (NBUF - 2) * (kLoads - kALoads) + kHalf + kSRows) // (all younger than step 0)
+                   (NBUF - 2) * (kLoads - kALoads) + kHalf + kLate) // (all younger than step 0)
                : "memory");
   read_frags(f0, 0, 0);
   read_scales(c0, 0);
@@ -936,30 +979,30 @@ AXH_MX_TYPES(AXH_MX_KSPLIT_GATE_UP, k32, false, 4, 3)
 AXH_MX_KSPLIT_GATE_UP(mxfp4, TF32, k32, true, 4, 3)
 
 // Tile kernels: NAME, rows and columns of the tile, waves along both and groups of
-// them along K, buffers of a group, waves of a SIMD.
-#define AXH_MX_TILE_DENSE(TN, T, NAME, BM, BN, WM, WN, WK, NBUF, WPE) \
+// them along K, buffers of a group, waves of a SIMD (and true: short rows).
+#define AXH_MX_TILE_DENSE(TN, T, NAME, BM, BN, WM, WN, WK, NBUF, WPE, ...) \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK)      \
       __attribute__((amdgpu_waves_per_eu(WPE, WPE)))              \
       axh_mxfp4_matmul_##NAME##_##TN(AXH_MX_DENSE_ARGS) {         \
     extern __shared__ __align__(16) uint8_t tile[];               \
     AXH_MX_DENSE_UNPACK;                                          \
-    tile_body<kDense, T, false, BM, BN, WM, WN, WK, NBUF>(a, tile);   \
+    tile_body<kDense, T, false, BM, BN, WM, WN, WK, NBUF __VA_OPT__(,) __VA_ARGS__>(a, tile);   \
   }
-#define AXH_MX_TILE_EXPERT(TN, T, NAME, BM, BN, WM, WN, WK, NBUF, WPE) \
+#define AXH_MX_TILE_EXPERT(TN, T, NAME, BM, BN, WM, WN, WK, NBUF, WPE, ...) \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK)       \
       __attribute__((amdgpu_waves_per_eu(WPE, WPE)))               \
       axh_mxfp4_expert_matmul_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {  \
     extern __shared__ __align__(16) uint8_t tile[];                \
     AXH_MX_EXPERT_UNPACK;                                          \
-    tile_body<kGrouped, T, false, BM, BN, WM, WN, WK, NBUF>(a, tile);  \
+    tile_body<kGrouped, T, false, BM, BN, WM, WN, WK, NBUF __VA_OPT__(,) __VA_ARGS__>(a, tile);  \
   }
-#define AXH_MX_TILE_GATE_UP(TN, T, NAME, PACKED, BM, BN, WM, WN, WK, NBUF, WPE) \
+#define AXH_MX_TILE_GATE_UP(TN, T, NAME, PACKED, BM, BN, WM, WN, WK, NBUF, WPE, ...) \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK)                \
       __attribute__((amdgpu_waves_per_eu(WPE, WPE)))                        \
       axh_mxfp4_expert_gate_up_##NAME##_##TN(AXH_MX_EXPERT_ARGS) {          \
     extern __shared__ __align__(16) uint8_t tile[];                         \
     AXH_MX_EXPERT_UNPACK;                                                   \
-    tile_body<kGateUp, T, PACKED, BM, BN, WM, WN, WK, NBUF>(a, tile);           \
+    tile_body<kGateUp, T, PACKED, BM, BN, WM, WN, WK, NBUF __VA_OPT__(,) __VA_ARGS__>(a, tile);           \
   }
 #define AXH_MX_TILE_EXPERTS(NAME, ...)                        \
   AXH_MX_TYPES(AXH_MX_TILE_EXPERT, NAME, __VA_ARGS__)         \
@@ -973,3 +1016,5 @@ AXH_MX_TYPES(AXH_MX_TILE_DENSE, t256x256, 256, 256, 2, 4, 1, 2, 2)
 AXH_MX_TILE_EXPERTS(t128x64, 128, 64, 2, 2, 1, 3, 2)
 AXH_MX_TILE_EXPERTS(t128x128, 128, 128, 2, 2, 1, 2, 2)
 AXH_MX_TILE_EXPERTS(t256x256, 256, 256, 2, 4, 1, 2, 2)
+AXH_MX_TYPES(AXH_MX_TILE_DENSE, t128x128n, 128, 128, 2, 2, 1, 2, 2, true)
+AXH_MX_TILE_EXPERTS(t128x128n, 128, 128, 2, 2, 1, 2, 2, true)

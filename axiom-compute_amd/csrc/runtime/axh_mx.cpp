@@ -113,6 +113,7 @@ struct MatmulKind {
 };
 constexpr MatmulKind k256x256 = {"t256x256", 256, 256, 512, 147456};
 constexpr MatmulKind k128x128 = {"t128x128", 128, 128, 256, 73728};
+constexpr MatmulKind k128x128Short = {"t128x128n", 128, 128, 256, 73728};
 constexpr MatmulKind k128x64 = {"t128x64", 128, 64, 256, 81920};
 constexpr MatmulKind k64x128 = {"t64x128", 64, 128, 256, 81920};
 constexpr MatmulKind k64x64 = {"t64x64", 64, 64, 128, 53248};
@@ -133,11 +134,15 @@ constexpr uint32_t kTileMinBlocks = 16; // the tiles read 16 scales of a row at 
 // columns, 6.6 against 7.1; 128 columns (512 tiles) 12.3 against 7.7; with half the rows
 // if K is long and those fit as well: 4096 x 14336, 32 columns, 13.9 against 16.3; 4096 x
 // 4096 7.6 against 6.6.
+// Rows of fewer than 16 blocks, through 128x128 against the K-split kernel, a layer of us:
+// 2894 tokens, 6 of 34 experts, 1536 x 352: 75.5 / 416; 3639 tokens, 7 of 72, 2048 x 256:
+// 110 / 838.
 const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
   auto grid = [&](const MatmulKind &k) {
     return (uint64_t)div_up(n_rows, k.rows) * div_up(batch, k.cols);
   };
-  if (nblk < kTileMinBlocks) return kSplit32;
+  if (nblk < kTileMinBlocks) // (a load of 16 scales has to stay inside both arrays)
+    return batch > 64u && n_rows >= 16u && grid(k128x128Short) >= 200u ? k128x128Short : kSplit32;
   if (batch > 128u && grid(k256x256) >= 200u) return k256x256;
   if (batch > 64u && grid(k128x128) >= 200u) return k128x128;
   if (batch > 64u && grid(k64x64) > 256u) return k64x128;
@@ -155,8 +160,9 @@ const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
 // 256: 190 / 90, 167 / 95; 8 experts, 4096 x 14336, mean 75: 124 / 65, 167 / 97; mean 175:
 // 234 / 89, 174 / 92.
 const MatmulKind &expert_kind(uint32_t n_rows, uint32_t nblk, uint64_t slots, uint32_t n_experts,
-                              bool gate_up) {
+                              uint32_t n_x, bool gate_up) {
   const uint64_t mean = slots / n_experts;
+  if (nblk < kTileMinBlocks && mean >= 64u && n_rows >= 16u && n_x >= 16u) return k128x128Short;
   if (nblk < kTileMinBlocks) return gate_up ? kSplit32GateUp : kSplit32;
   if (mean <= 52u) return k128x64;
   return mean >= 160u && mean * n_rows >= 1u << 19 ? k256x256 : k128x128;
@@ -187,7 +193,7 @@ axh_status expert_launch(axh_context *ctx, const char *op, const char *type, boo
                          uint32_t x_div, uint64_t slots, uint32_t n_experts, void *stream) {
   if ((uint64_t)n_x * (cols / 2u) >= kMaxBuffer)
     return bad("the activations' codes must be below 2 GiB");
-  const MatmulKind &k = expert_kind(n_rows, cols / 32u, slots, n_experts, gate_up);
+  const MatmulKind &k = expert_kind(n_rows, cols / 32u, slots, n_experts, n_x, gate_up);
   // the experts' last tiles are partial: at most so many tiles in all
   const uint64_t active = std::min<uint64_t>(n_experts, slots);
   const uint64_t tiles = active + (slots - active) / k.cols;

@@ -675,6 +675,24 @@ def test_expert_down_and_combine(ctx, dev, axc, tokens, top_k, n, hidden, ffn, t
         2.0 ** -25 if t == F16 else 0)).all()
 
 
+# rows of fewer than 16 blocks through the 128 x 128 tiles: matrices, prompts, blocks 1 to 15
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,cols,batch", [(2000, 32, 1700), (1801, 256, 1665), (2000, 288, 1700),
+                                             (3500, 480, 900)])
+def test_matmul_short_rows(ctx, dev, axc, rows, cols, batch, t):
+    assert "_t128x128n_" in axc.mxfp4_matmul_kernel_name(rows, cols, batch, t)
+    test_matmul(ctx, dev, axc, rows, cols, batch, t)
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16, MXFP4])
+@pytest.mark.parametrize("tokens,top_k,n,hidden,ffn", [(700, 2, 8, 96, 160), (400, 3, 5, 480, 32),
+                                                       (260, 1, 3, 256, 288)])
+def test_expert_products_short_rows(ctx, dev, axc, tokens, top_k, n, hidden, ffn, t):
+    test_expert_products_for_prompts(ctx, dev, axc, tokens, top_k, n, hidden, ffn, t)
+    if t != MXFP4:
+        test_expert_down_and_combine(ctx, dev, axc, tokens, top_k, n, hidden, ffn, t)
+
+
 @pytest.mark.parametrize("cols", [1, 7, 33, 2049, 4096])
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 def test_combine_odd_columns(ctx, dev, cols, t):

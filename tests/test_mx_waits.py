@@ -19,7 +19,7 @@ import pytest
 OBJDUMP = shutil.which("llvm-objdump") or "/opt/rocm/llvm/bin/llvm-objdump"
 # tile -> loads of a wave and step, of them of A, and buffers
 TILES = {"t64x64": (8, 4, 3), "t64x64s2": (8, 4, 3), "t64x128": (6, 2, 3), "t128x64": (6, 4, 3),
-         "t128x128": (8, 4, 2), "t256x256": (8, 4, 2)}
+         "t128x128": (8, 4, 2), "t128x128n": (8, 4, 2), "t256x256": (8, 4, 2)}
 
 
 @pytest.fixture(scope="module")
