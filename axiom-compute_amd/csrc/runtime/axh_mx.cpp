@@ -136,7 +136,8 @@ constexpr uint32_t kTileMinBlocks = 16; // the tiles read 16 scales of a row at 
 // 4096 7.6 against 6.6.
 // Rows of fewer than 16 blocks, through 128x128 against the K-split kernel, a layer of us:
 // 2894 tokens, 6 of 34 experts, 1536 x 352: 75.5 / 416; 3639 tokens, 7 of 72, 2048 x 256:
-// 110 / 838.
+// 110 / 838; 30 experts, 2048 x 480, mean 4: 24 / 41, mean 60: 32 / 88; 64, 1536 x 256,
+// mean 4: 26 / 52, mean 60: 38 / 122.
 const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
   auto grid = [&](const MatmulKind &k) {
     return (uint64_t)div_up(n_rows, k.rows) * div_up(batch, k.cols);
@@ -162,8 +163,10 @@ const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
 const MatmulKind &expert_kind(uint32_t n_rows, uint32_t nblk, uint64_t slots, uint32_t n_experts,
                               uint32_t n_x, bool gate_up) {
   const uint64_t mean = slots / n_experts;
-  if (nblk < kTileMinBlocks && mean >= 64u && n_rows >= 16u && n_x >= 16u) return k128x128Short;
-  if (nblk < kTileMinBlocks) return gate_up ? kSplit32GateUp : kSplit32;
+  if (nblk < kTileMinBlocks) { // (a load of 16 scales has to stay inside both arrays)
+    if (n_rows >= 16u && n_x >= 16u) return k128x128Short;
+    return gate_up ? kSplit32GateUp : kSplit32;
+  }
   if (mean <= 52u) return k128x64;
   return mean >= 160u && mean * n_rows >= 1u << 19 ? k256x256 : k128x128;
 }
