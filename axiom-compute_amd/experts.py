@@ -11,7 +11,9 @@ Tensors are those of a GGUF layer `prefix`: ffn_gate_exps.weight and
 ffn_up_exps.weight (hidden x ffn x experts, ne[0] first), ffn_down_exps.weight (ffn x
 hidden x experts), of type MXFP4; the router's ffn_gate_inp.weight (hidden x experts), f32,
 f16 or bf16 (its product is in f32 then), or MXFP4; and exp_probs_b.bias (experts, f32)
-where the router adds a bias to its choices.
+where the router adds a bias to its choices.  What is computed is y = sum over a token's
+choices of weight * (down (silu(gate x) * (up x))): a file whose layer holds more than that
+(biases of the experts' or the router's products, shared experts) is refused.
 
 The codes and scales are laid out once, when the layer is made, and so are the
 workspaces: run() allocates nothing and can be captured in a graph.  No counterpart
@@ -19,12 +21,21 @@ in the reference, which has no expert layers.
 """
 from __future__ import annotations
 
-from typing import Optional
+import re
+from typing import Iterable, Optional
 
 from . import axh as _axh
 from .gguf import GGML_MXFP4, GgufFile
 
 GGML_F32 = 0
+
+
+def _unused(file: GgufFile, prefix: str, used: Iterable[str]) -> list[str]:
+    """Tensors of the router or the experts that are not used: all that are called ffn_* or
+    exp_* but norms (of the layer's input) and a dense feed-forward beside the experts."""
+    part = re.compile(re.escape(prefix) + r"\.(?!ffn_norm|ffn_post_norm|ffn_(gate|up|down)\.)"
+                      r"(ffn_|exp_)")
+    return sorted(n for n in file.tensors if part.match(n) and n not in used)
 
 
 class _Matrix:
@@ -70,10 +81,16 @@ class ExpertLayer:
     quantised to MXFP4 and grouped by expert.  The default is three choices for four
     experts, about where the times cross (us): 64 experts, 8 choices, 2048 x 1024, 6
     tokens 36 / 45, 12 tokens 58 / 54; 32, 4, 4096 x 1408, 6 tokens 50 / 51; 8, 2, 4096 x
-    14336, 2 tokens 71 / 90, 4 tokens 131 / 109."""
+    14336, 2 tokens 71 / 90, 4 tokens 131 / 109.
+
+    The gate's activation is `activation`, of which "silu" is the only one there is.  A tensor
+    of the layer that run() does not use is a ValueError, as the layer would be another one
+    without it; leave_out names those (without the prefix) that the caller computes itself,
+    such as shared experts whose output it adds."""
 
     def __init__(self, ctx, file: GgufFile, prefix: str, options: "_axh.RouteOptions",
-                 max_tokens: int, few_tokens: Optional[int] = None):
+                 max_tokens: int, few_tokens: Optional[int] = None, activation: str = "silu",
+                 leave_out: Iterable[str] = ()):
         if max_tokens < 1:
             raise ValueError("max_tokens must be at least 1")
         self.ctx, self.options = ctx, options
@@ -85,6 +102,13 @@ class ExpertLayer:
         for n in names.values():
             if n not in file.tensors:
                 raise ValueError(f"the file has no tensor {n}")
+        if activation != "silu":
+            raise ValueError(f"unknown activation {activation!r}")
+        bias = f"{prefix}.exp_probs_b.bias"
+        unused = _unused(file, prefix, {*names.values(), bias,
+                                        *(f"{prefix}.{n}" for n in leave_out)})
+        if unused:
+            raise ValueError(f"the layer has tensors that are not computed: {', '.join(unused)}")
         shapes = {n: tuple(file.tensors[t].shape) for n, t in names.items()}
         hidden, n = shapes["ffn_gate_inp"]
         ffn = shapes["ffn_gate_exps"][1]
@@ -98,7 +122,6 @@ class ExpertLayer:
         self.gate, self.up, self.down = (
             _Matrix(ctx, file, names[k]) for k in ("ffn_gate_exps", "ffn_up_exps",
                                                    "ffn_down_exps"))
-        bias = f"{prefix}.exp_probs_b.bias"
         self.bias = None
         if bias in file.tensors:
             t = file.tensors[bias]

@@ -237,3 +237,55 @@ def test_drawn_cases_are_within_the_operators_limits(cases):
             assert c["top_k"] <= c["groups_kept"] * (c["experts"] // c["groups"])
         for k in ("cols", "hidden", "ffn"):
             assert c.get(k, 32) % 32 == 0
+
+
+def _layer_file(axc, path, *more):
+    """The layer blk.3 in the smallest sizes, of zeros, and f32 tensors called `more`."""
+    n, hidden, ffn = 4, 64, 32
+    shapes = [("ffn_gate_inp.weight", (hidden, n)), ("ffn_gate_exps.weight", (hidden, ffn, n)),
+              ("ffn_up_exps.weight", (hidden, ffn, n)), ("ffn_down_exps.weight", (ffn, hidden, n))]
+    tensors = [(f"blk.3.{name}", axc.gguf.GGML_MXFP4, s, bytes(int(np.prod(s)) // 32 * 17))
+               for name, s in shapes]
+    axc.gguf.write_gguf(path, [], tensors + [(name, axc.gguf.GGML_F32, (n,), bytes(4 * n))
+                                             for name in more])
+
+
+@pytest.mark.parametrize("name", ["ffn_gate_inp.bias", "ffn_gate_exps.bias", "ffn_up_exps.bias",
+                                  "ffn_down_exps.bias", "ffn_up_exps.scale",
+                                  "ffn_gate_inp_shexp.weight", "ffn_gate_shexp.weight",
+                                  "ffn_up_shexp.weight", "ffn_down_shexp.weight",
+                                  "ffn_gate_chexps.weight", "exp_probs_b.weight"])
+def test_expert_layer_refuses_tensors_that_it_does_not_compute(axc, tmp_path, name):
+    """Before anything is put on the device (there is none here)."""
+    options = axc.RouteOptions(n_experts=4, top_k=1)
+    _layer_file(axc, tmp_path / "layer.gguf", f"blk.3.{name}")
+    with axc.gguf.GgufFile(tmp_path / "layer.gguf") as f:
+        with pytest.raises(ValueError, match=f"not computed: blk.3.{name}"):
+            axc.experts.ExpertLayer(None, f, "blk.3", options, max_tokens=8)
+        # another name does not stand for it, its own does: then the device is asked for
+        with pytest.raises(ValueError, match="not computed"):
+            axc.experts.ExpertLayer(None, f, "blk.3", options, max_tokens=8,
+                                    leave_out=["ffn_gate_inp"])
+        with pytest.raises(AttributeError):
+            axc.experts.ExpertLayer(None, f, "blk.3", options, max_tokens=8, leave_out=[name])
+
+
+def test_expert_layer_takes_what_stands_beside_it(axc, tmp_path):
+    """Norms, a dense feed-forward, attention and other layers' tensors are no part of it."""
+    options = axc.RouteOptions(n_experts=4, top_k=1)
+    _layer_file(axc, tmp_path / "layer.gguf", "blk.3.ffn_norm.weight",
+                "blk.3.ffn_norm_exps.weight", "blk.3.ffn_post_norm.weight",
+                "blk.3.ffn_gate.weight", "blk.3.ffn_up.weight", "blk.3.ffn_down.bias",
+                "blk.3.attn_q.bias", "blk.4.ffn_up_exps.bias", "blk.31.ffn_gate_inp.bias",
+                "blk.3.exp_probs_b.bias")
+    with axc.gguf.GgufFile(tmp_path / "layer.gguf") as f:
+        with pytest.raises(AttributeError):  # the device, which is None
+            axc.experts.ExpertLayer(None, f, "blk.3", options, max_tokens=8)
+
+
+def test_expert_layer_refuses_another_activation(axc, tmp_path):
+    _layer_file(axc, tmp_path / "layer.gguf")
+    with axc.gguf.GgufFile(tmp_path / "layer.gguf") as f:
+        with pytest.raises(ValueError, match="activation"):
+            axc.experts.ExpertLayer(None, f, "blk.3", axc.RouteOptions(n_experts=4, top_k=1),
+                                    max_tokens=8, activation="gelu")
