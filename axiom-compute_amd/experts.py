@@ -59,13 +59,21 @@ class _Matrix:
 
 
 class _Router:
-    """The router's matrix: f32, f16 or bf16 as it stands in the file, or MXFP4."""
+    """The router's matrix: f32, f16 or bf16 as it stands in the file, or MXFP4 (in_f32: decoded
+    to f32, which holds its values exactly)."""
 
-    def __init__(self, ctx, file: GgufFile, name: str):
+    def __init__(self, ctx, file: GgufFile, name: str, in_f32: bool):
         t = file.tensors[name]
         self.type, self.packed = t.type, None
         if t.type == GGML_MXFP4:
             self.packed = _Matrix(ctx, file, name)
+            if in_f32:
+                packed, self.packed, self.type = self.packed, None, GGML_F32
+                blocks = t.nbytes // 17
+                self.w = ctx.alloc(blocks * 128)
+                ctx.mxfp4_dequant(packed.codes, packed.scales, self.w, blocks, GGML_F32)
+                ctx.synchronize()
+                packed.close()
         elif t.type in (_axh.GGML_F32, _axh.GGML_F16, _axh.GGML_BF16):
             self.w = file.upload(ctx, name)
         else:
@@ -81,7 +89,14 @@ class ExpertLayer:
     quantised to MXFP4 and grouped by expert.  The default is three choices for four
     experts, about where the times cross (us): 64 experts, 8 choices, 2048 x 1024, 6
     tokens 36 / 45, 12 tokens 58 / 54; 32, 4, 4096 x 1408, 6 tokens 50 / 51; 8, 2, 4096 x
-    14336, 2 tokens 71 / 90, 4 tokens 131 / 109.
+    14336, 2 tokens 71 / 90, 4 tokens 131 / 109.  So the precision of a token's activations
+    depends on how many tokens come with it, unless few_tokens is 0 (all in MXFP4) or
+    max_tokens (all in f32).
+
+    A router in MXFP4 multiplies one token's activations in f32 and those of several in MXFP4,
+    so that even the choice of a token's experts may depend on the others.  With router_f32 its
+    matrix is decoded once and the product is in f32 for any number of tokens, as it is for
+    routers in f32, f16 or bf16 without it.
 
     The gate's activation is `activation`, of which "silu" is the only one there is.  A tensor
     of the layer that run() does not use is a ValueError, as the layer would be another one
@@ -90,7 +105,7 @@ class ExpertLayer:
 
     def __init__(self, ctx, file: GgufFile, prefix: str, options: "_axh.RouteOptions",
                  max_tokens: int, few_tokens: Optional[int] = None, activation: str = "silu",
-                 leave_out: Iterable[str] = ()):
+                 leave_out: Iterable[str] = (), router_f32: bool = False):
         if max_tokens < 1:
             raise ValueError("max_tokens must be at least 1")
         self.ctx, self.options = ctx, options
@@ -118,7 +133,7 @@ class ExpertLayer:
             raise ValueError(f"the tensors' shapes do not make a layer of {options.n_experts} "
                              f"experts: {shapes}")
         self.hidden, self.ffn = hidden, ffn
-        self.router = _Router(ctx, file, names["ffn_gate_inp"])
+        self.router = _Router(ctx, file, names["ffn_gate_inp"], router_f32)
         self.gate, self.up, self.down = (
             _Matrix(ctx, file, names[k]) for k in ("ffn_gate_exps", "ffn_up_exps",
                                                    "ffn_down_exps"))
