@@ -6,8 +6,8 @@ into libaxh.so (hand-written HIP kernels + C ABI runtime).
 """
 from . import axh, experts, gguf  # noqa: F401
 from .axh import (  # noqa: F401
-    FAMILY_COLUMNS, FAMILY_DEFAULT, FAMILY_ONE_PASS, FAMILY_ONE_PASS_X, FAMILY_PERSISTENT,
-    FAMILY_SPLIT_K, FAMILY_TILED, FAMILY_WORKGROUP, BindingPlan, DeviceBuffer, DispatchError,
+    DEFAULT_STREAM, FAMILY_COLUMNS, FAMILY_DEFAULT, FAMILY_ONE_PASS, FAMILY_ONE_PASS_X,
+    FAMILY_PERSISTENT, FAMILY_SPLIT_K, FAMILY_TILED, FAMILY_WORKGROUP, BindingPlan, DeviceBuffer, DispatchError,
     DispatchRequest, Graph, HipContext, HipContextOptions, KernelHandle, MatmulVariant,
     RouteOptions, Variant, builtin_code_object, compiled_matmul_variants, compiled_variants,
     expert_plan_bytes, ggml_type_size, load_library, mxfp4_matmul_kernel_name,

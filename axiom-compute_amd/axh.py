@@ -127,6 +127,9 @@ class _RouteOptions(ctypes.Structure):
                 ("normalize", ctypes.c_uint32), ("scale", ctypes.c_float)]
 
 
+# The default stream of this library's HIP runtime as a `stream` argument (AXH_STREAM_DEFAULT).
+DEFAULT_STREAM = 1
+
 # Element types of the MXFP4 and expert operations (ggml type ids).
 GGML_F32, GGML_F16, GGML_BF16, GGML_MXFP4 = 0, 1, 30, 39
 SCORES = {"softmax": 0, "sigmoid": 1}
@@ -577,7 +580,8 @@ def _ptr(obj) -> int:
 
 
 def _stream(s) -> Optional[int]:
-    """A hipStream_t of this library's HIP runtime, as an int (None = context stream)."""
+    """A hipStream_t of this library's HIP runtime, as an int (None and 0: the context's own
+    stream, which is not ordered with the runtime's default stream; DEFAULT_STREAM: that one)."""
     if s is None:
         return None
     if isinstance(s, int):

@@ -57,6 +57,7 @@ Core::~Core() {
 }
 
 hipStream_t pick_stream(axh_context *ctx, void *stream) {
+  if (stream == AXH_STREAM_DEFAULT) return nullptr; // HIP's handle of it
   return stream ? static_cast<hipStream_t>(stream) : ctx->core->stream;
 }
 

@@ -6,7 +6,9 @@
  * axh_status and leaves a thread-local message readable with axh_last_error().
  * Device pointers are HIP device addresses (from axh_buffer_alloc or any other
  * HIP allocation on the context's device).  `stream` arguments are hipStream_t
- * values passed as void*; NULL means the context's own stream.
+ * values passed as void*; NULL means the context's own stream, which is ordered
+ * with no other, the device's default stream included; that one is
+ * AXH_STREAM_DEFAULT.
  */
 #ifndef AXH_H
 #define AXH_H
@@ -17,6 +19,11 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* The device's default stream as a `stream` argument (its handle in HIP is 0, which
+ * here means the context's own): for memory that others in this HIP runtime fill,
+ * read or reuse in the order of that stream. */
+#define AXH_STREAM_DEFAULT ((void *)1)
 
 /* Layout version of the structs below, raised whenever one of them changes
  * size or field order.  2: axh_q4_variant grew from 4 to 6 fields (16 to 24
