@@ -400,6 +400,8 @@ axh_status axh_expert_route(axh_context *ctx, uint32_t logits_type, const void *
     if (o->groups_kept == 0 || o->groups_kept > groups)
       return bad("groups_kept must be 1 to n_groups");
     if (o->group_best != 1u && o->group_best != 2u) return bad("group_best must be 1 or 2");
+    if (o->group_best > o->n_experts / groups)
+      return bad("groups of one expert have no two best: group_best must be 1");
     if ((uint64_t)o->groups_kept * (o->n_experts / groups) < o->top_k)
       return bad("the kept groups hold fewer experts than top_k");
   }

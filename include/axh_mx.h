@@ -77,10 +77,11 @@ axh_status axh_expert_logits(axh_context *ctx, uint32_t w_type, const void *w, c
  * token's logits or the sigmoid of its logit; the order is by key, the score
  * plus the expert's bias (f32, NULL for none), the lowest expert first among
  * equals.  With groups (n_groups > 1, dividing n_experts, at most 64), a
- * group's key is its best key or the sum of its two best (group_best 1 or 2),
- * the groups_kept best groups are kept, and choices come from them only.  The
- * weight of a choice is its score, without the bias, divided by the sum over
- * the token's choices where normalize is set, times scale.
+ * group's key is its best key or the sum of its two best (group_best 1, or 2 in
+ * groups of at least two experts), the groups_kept best groups are kept, and
+ * choices come from them only.  The weight of a choice is its score, without the
+ * bias, divided by the sum over the token's choices where normalize is set, times
+ * scale.
  *   Scores are f32 (a sigmoid below its range is 0; choices whose scores add up
  * to 0 have weight 0).  Keys are compared as f32; where only the order of single scores counts (no
  * bias, and one group or group_best 1) the logits themselves are compared.
