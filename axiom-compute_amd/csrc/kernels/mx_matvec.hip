@@ -46,6 +46,15 @@ __device__ __forceinline__ f32x2_t swap16_f(float a, float b) {
   return (f32x2_t){__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
 }
 
+// silu(g) * u on the library's exponential and an exact quotient, as the gate/up kernels of
+// the other formats have it: within 3 ulp, and 0 from g = -88.72 on, where the exponential is
+// beyond f32.  One a row, after the sums, so that it costs next to nothing (1 token, 8 of 64
+// experts, 2048 x 1024: 6.80 us against 6.74 with swiglu of mx_common.h, which prompts take,
+// as its fewer instructions count there).
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  return g / (1.0f + expf(-g)) * u;
+}
+
 // The sum over the 16 lanes of a DPP row, in all of them.
 __device__ __forceinline__ float row_sum16(float v) {
   v += dpp_f32<kXor1>(v);
@@ -253,7 +262,7 @@ matvec_body(const uint8_t *wc, const uint8_t *ws, const uint8_t *wc2, const uint
       const float *q = p + group_rows * a.uw;
       float up = 0.0f;
       for (uint32_t u = 0; u < a.uw; ++u) up += q[u];
-      sum = swiglu(sum, up);
+      sum = silu_mul(sum, up);
     }
     y[(uint64_t)item * a.n_rows + row] = sum;
   }

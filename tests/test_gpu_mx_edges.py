@@ -210,6 +210,26 @@ def test_gates_over_the_range_of_silu(ctx, dev, axc, prompt, cols, up_scale):
     assert (np.abs(h - want) <= bound).all()
 
 
+def test_gates_of_few_tokens_are_exact_to_three_ulp(ctx, dev):
+    """f32's exponential (1 ulp), an addition, a quotient and a product (half each), until the
+    exponential of -g is beyond f32: below g = -88.72, silu(g) is within 2.7e-37."""
+    cols = 576
+    g, u = _gates()
+    rows = len(g)
+    gc, gs = _matrix(g, cols)
+    uc, us = _matrix(u, cols, 60)
+    u = u * 2.0 ** 60
+    dh = dev.out(rows * 4)
+    ctx.mxfp4_expert_gate_up(dev.up(gc), dev.up(gs), dev.up(uc), dev.up(us),
+                             dev.up(np.ones((1, cols), dtype=np.float32)),
+                             dev.up(np.zeros((1, 1), dtype=np.int32)), dh, rows, cols, 1, 1, 1)
+    ctx.synchronize()
+    h = dev.down(dh, rows * 4, np.float32, rows).astype(np.float64)
+    want = MX.swiglu(g, u)
+    bound = 3 * U23 * np.abs(want) + np.where(g < -88.72, 2.7e-37, 0) * np.abs(u) + 2.0 ** -148
+    assert (np.abs(h - want) <= bound).all()
+
+
 def test_infinite_gates_for_few_tokens(ctx, dev):
     """g beyond f32 is an infinity: silu(inf) is inf, silu(-inf) the formula's NaN, and neither
     reaches another row."""
