@@ -134,16 +134,17 @@ constexpr uint32_t kTileMinBlocks = 16; // the tiles read 16 scales of a row at 
 // columns, 6.6 against 7.1; 128 columns (512 tiles) 12.3 against 7.7; with half the rows
 // if K is long and those fit as well: 4096 x 14336, 32 columns, 13.9 against 16.3; 4096 x
 // 4096 7.6 against 6.6.
-// Rows of fewer than 16 blocks, through 128x128 against the K-split kernel, a layer of us:
-// 2894 tokens, 6 of 34 experts, 1536 x 352: 75.5 / 416; 3639 tokens, 7 of 72, 2048 x 256:
-// 110 / 838; 30 experts, 2048 x 480, mean 4: 24 / 41, mean 60: 32 / 88; 64, 1536 x 256,
-// mean 4: 26 / 52, mean 60: 38 / 122.
+// Rows of fewer than 16 blocks: the K-split kernel where its tiles are one round, else 128x128.
+// bf16 y, us, K-split / 128x128: 1536 x 256, 128 columns (192 tiles) 3.5 / 4.2, 256 columns
+// (384) 5.7 / 4.3, 2000 columns 27.9 / 5.1; 8192 x 480, 32 columns (256) 3.7 / 4.0, 64 columns
+// (512) 6.1 / 4.4; 16384 x 32, 16 columns (512) 4.4 / 4.1; 32 x 480, 4096 columns (128) 3.6 /
+// 4.2; 2880 x 32, 128 columns (360) 4.5 / 4.3.
 const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
   auto grid = [&](const MatmulKind &k) {
     return (uint64_t)div_up(n_rows, k.rows) * div_up(batch, k.cols);
   };
   if (nblk < kTileMinBlocks) // (a load of 16 scales has to stay inside both arrays)
-    return batch > 64u && n_rows >= 16u && grid(k128x128Short) >= 200u ? k128x128Short : kSplit32;
+    return batch >= 16u && n_rows >= 16u && grid(kSplit32) > 256u ? k128x128Short : kSplit32;
   if (batch > 128u && grid(k256x256) >= 200u) return k256x256;
   if (batch > 64u && grid(k128x128) >= 200u) return k128x128;
   if (batch > 64u && grid(k64x64) > 256u) return k64x128;
@@ -160,6 +161,10 @@ const MatmulKind &dense_kind(uint32_t n_rows, uint32_t nblk, uint32_t batch) {
 // 1024, mean 256: 47.8 / 32.5, 53 / 33.2; mean 512: 77 / 49.5, 71 / 48; 2880 x 2880, mean
 // 256: 190 / 90, 167 / 95; 8 experts, 4096 x 14336, mean 75: 124 / 65, 167 / 97; mean 175:
 // 234 / 89, 174 / 92.
+// Rows of fewer than 16 blocks, through 128x128 against the K-split kernel, a layer of us:
+// 2894 tokens, 6 of 34 experts, 1536 x 352: 75.5 / 416; 3639 tokens, 7 of 72, 2048 x 256:
+// 110 / 838; 30 experts, 2048 x 480, mean 4: 24 / 41, mean 60: 32 / 88; 64, 1536 x 256,
+// mean 4: 26 / 52, mean 60: 38 / 122.
 const MatmulKind &expert_kind(uint32_t n_rows, uint32_t nblk, uint64_t slots, uint32_t n_experts,
                               uint32_t n_x, bool gate_up) {
   const uint64_t mean = slots / n_experts;

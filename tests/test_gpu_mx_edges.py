@@ -11,7 +11,8 @@ import numpy as np
 import pytest
 
 from oracle import mx_numpy as MX
-from test_gpu_mx import F32, MXFP4, U23, Dev, _choices, _say, activations
+import test_gpu_mx
+from test_gpu_mx import BF16, F16, F32, MXFP4, U23, Dev, _choices, _say, activations
 
 pytestmark = pytest.mark.gpu
 
@@ -248,3 +249,15 @@ def test_infinite_gates_for_few_tokens(ctx, dev):
     rest = np.delete(h, [5, 6])
     want = float(MX.swiglu(np.float64(1), np.float64(2)))
     assert (np.abs(rest - want) <= 8 * U23 * want).all()
+
+
+# ---- short rows on 128 x 128 tiles in the smallest arrays that they are taken for -------------
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,cols,batch", [(16, 32, 8224), (8224, 32, 16), (16, 480, 8224),
+                                             (8208, 256, 17), (4100, 288, 70)])
+def test_small_products_of_short_rows(ctx, dev, axc, rows, cols, batch, t):
+    assert "_t128x128n_" in axc.mxfp4_matmul_kernel_name(rows, cols, batch, t)
+    test_gpu_mx.test_matmul(ctx, dev, axc, rows, cols, batch, t)
+    if t == F32:
+        test_nan_blocks_of_a_product_stay_in_their_rows(ctx, dev, axc, rows, cols, batch,
+                                                        "t128x128n")
