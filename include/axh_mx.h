@@ -110,7 +110,8 @@ axh_status axh_expert_route(axh_context *ctx, uint32_t logits_type, const void *
  * experts: n_tokens x top_k int32 as from axh_expert_route; choice k of token t
  * is slot t * top_k + k.  Choices outside 0 .. n_experts - 1 are left out.  The
  * experts' matrices follow one another (n_experts x n_rows x cols), each below
- * 2 GiB of codes.
+ * 2 GiB of codes.  silu(g) * u is within 3 ulp, 0 from g = -88.72 down, for few
+ * tokens, and within 5 ulp, 0 from g = -87.3 down, for prompts.
  *
  * Few tokens, f32 activations, every chosen expert's weights read once a slot:
  *   gate_up: h[slot] = silu(Wg[e] x[t]) * (Wu[e] x[t]), slots x n_rows f32 (0
@@ -154,7 +155,8 @@ axh_status axh_mxfp4_expert_matmul(axh_context *ctx, const void *codes, const vo
                                    void *stream);
 /* y[t] = sum over choices of weight * slots[slot], in f32 in the choices'
  * order, rounded once; slots and y of one type (f32, f16 or bf16), both 16-byte
- * aligned.  n_experts 0 leaves out negative choices only. */
+ * aligned.  (Slots of 16 bits are rounded once more, when they are written: in
+ * bf16 the error of y is 0.0024 by norm, 0.0017 for f32 slots whose sum is rounded.)  n_experts 0 leaves out negative choices only. */
 axh_status axh_expert_combine(axh_context *ctx, uint32_t y_type, const void *slots,
                               const int32_t *experts, const float *weights, void *y,
                               uint32_t n_rows, uint32_t n_tokens, uint32_t top_k,
