@@ -155,8 +155,9 @@ axh_status axh_mxfp4_expert_matmul(axh_context *ctx, const void *codes, const vo
                                    void *stream);
 /* y[t] = sum over choices of weight * slots[slot], in f32 in the choices'
  * order, rounded once; slots and y of one type (f32, f16 or bf16), both 16-byte
- * aligned.  (Slots of 16 bits are rounded once more, when they are written: in
- * bf16 the error of y is 0.0024 by norm, 0.0017 for f32 slots whose sum is rounded.)  n_experts 0 leaves out negative choices only. */
+ * aligned.  Slots of 16 bits were rounded once more when they were written: in
+ * bf16 the error of y is 0.0024 by norm, 0.0017 for f32 slots whose sum is then
+ * rounded.  n_experts 0 leaves out negative choices only. */
 axh_status axh_expert_combine(axh_context *ctx, uint32_t y_type, const void *slots,
                               const int32_t *experts, const float *weights, void *y,
                               uint32_t n_rows, uint32_t n_tokens, uint32_t top_k,
