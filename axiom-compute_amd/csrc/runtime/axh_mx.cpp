@@ -55,7 +55,8 @@ axh_status check_cols(uint32_t cols) {
 axh_status launch(axh_context *ctx, Object obj, const std::string &name, uint64_t gx, uint64_t gy,
                   uint32_t threads, uint32_t lds, void *const *bufs, uint32_t n_bufs,
                   const uint32_t *words, uint32_t n_words, void *stream) {
-  if (gx > ctx->core->max_wg[0] || gy > ctx->core->max_wg[1])
+  // (a dimension's work-items are counted in 32 bits)
+  if (gx > ctx->core->max_wg[0] || gy > ctx->core->max_wg[1] || gx * threads > UINT32_MAX)
     return fail(AXH_ERR_WORKGROUP_COUNT_EXCEEDS_LIMIT, name + ": grid exceeds the device limit");
   hipSetDevice(ctx->core->device);
   axh_kernel *k = nullptr;

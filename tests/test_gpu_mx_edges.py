@@ -261,3 +261,19 @@ def test_small_products_of_short_rows(ctx, dev, axc, rows, cols, batch, t):
     if t == F32:
         test_nan_blocks_of_a_product_stay_in_their_rows(ctx, dev, axc, rows, cols, batch,
                                                         "t128x128n")
+
+
+def test_launches_of_more_work_items_than_a_dimension_has(ctx, dev, axc):
+    """2^32 of them or more are a typed error on the host, before any launch: the buffers here
+    are far smaller than such calls' and stay as they were."""
+    p = dev.out(1 << 12)
+    for call in (lambda: ctx.expert_combine(p, p, p, p, 8, 1 << 24, 1),
+                 lambda: ctx.mxfp4_dequant(p, p, p, (1 << 30) - 1),
+                 lambda: ctx.mxfp4_unpack_ggml(p, p, p, (1 << 30) - 63),
+                 lambda: ctx.expert_route(p, None, p, p, 1 << 26, axc.RouteOptions(4, 1)),
+                 lambda: ctx.mxfp4_matmul(p, p, p, p, p, 1 << 31, 32, 1)):
+        with pytest.raises(axc.DispatchError) as err:
+            call()
+        assert err.value.variant == "WorkgroupCountExceedsDeviceLimit"
+    ctx.synchronize()
+    assert (dev.down(p, 1 << 12, np.uint8, (1 << 12,)) == 0xA5).all()
