@@ -13,9 +13,10 @@
  * same with the sign bit (8) set.  A rows x cols matrix (cols a multiple of 32,
  * at most 2^22) is two arrays: codes, rows x cols / 2 bytes, the even element in
  * the low nibble, 16-byte aligned; and scales, rows x cols / 32 bytes, of any
- * alignment.  A call takes fewer than 2^30 - 64 blocks of 32 to quantise, decode or
- * unpack, and at most 2^24 - 1 tokens to sum up.  Element types of other operands are ggml type ids: AXH_GGML_F32,
- * AXH_GGML_F16 or AXH_GGML_BF16, and AXH_GGML_MXFP4 where it is said.
+ * alignment.  A call quantises, decodes or unpacks at most 2^30 - 64 blocks of 32,
+ * and sums up the choices of at most 2^24 - 1 tokens.  Element types of other
+ * operands are ggml type ids: AXH_GGML_F32, AXH_GGML_F16 or AXH_GGML_BF16, and
+ * AXH_GGML_MXFP4 where it is said.
  */
 #ifndef AXH_MX_H
 #define AXH_MX_H
