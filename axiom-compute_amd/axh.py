@@ -127,12 +127,41 @@ class _RouteOptions(ctypes.Structure):
                 ("normalize", ctypes.c_uint32), ("scale", ctypes.c_float)]
 
 
+class _RopeOptions(ctypes.Structure):
+    _fields_ = [("dim", ctypes.c_uint32), ("layout", ctypes.c_uint32), ("base", ctypes.c_double),
+                ("scale", ctypes.c_double), ("extrapolate", ctypes.c_double),
+                ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double),
+                ("original", ctypes.c_uint32), ("magnitude", ctypes.c_float)]
+
+
+class _Rope(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("dim", ctypes.c_uint32), ("layout", ctypes.c_uint32)]
+
+
+class _KvCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_pages", ctypes.c_uint32),
+                ("page_size", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32)]
+
+
+class _KvBatch(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32),
+                ("max_pages", ctypes.c_uint32), ("starts", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("table", ctypes.c_void_p)]
+
+
+class _AttentionOptions(ctypes.Structure):
+    _fields_ = [("n_heads", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("window", ctypes.c_uint32), ("max_length", ctypes.c_uint32)]
+
+
 # The default stream of this library's HIP runtime as a `stream` argument (AXH_STREAM_DEFAULT).
 DEFAULT_STREAM = 1
 
 # Element types of the MXFP4 and expert operations (ggml type ids).
 GGML_F32, GGML_F16, GGML_BF16, GGML_MXFP4 = 0, 1, 30, 39
 SCORES = {"softmax": 0, "sigmoid": 1}
+ROPE_LAYOUTS = {"pairs": 0, "halves": 1}
 
 BENCH_OPS = {"q4k": 1, "q4_0": 2, "q5k": 3, "q6k": 4, "gate_up": 5, "matmul_f16": 6,
              "matmul_f32": 7, "read_floor": 8, "launch_empty": 9, "read_shape": 10,
@@ -279,6 +308,19 @@ def load_library(path: Optional[Path] = None) -> ctypes.CDLL:
         "axh_mxfp4_expert_matmul": (st, [vp, vp, vp, vp, vp, vp, u32, vp, u32, u32, u32, u32, u32,
                                          vp]),
         "axh_expert_combine": (st, [vp, u32, vp, vp, vp, vp, u32, u32, u32, u32, vp]),
+        "axh_rope_table_bytes": (u64, [u32]),
+        "axh_rope_table": (st, [vp, c.POINTER(_RopeOptions), c.POINTER(c.c_float), vp]),
+        "axh_rope_apply": (st, [vp, u32, vp, u64, vp, u64, vp, u32, u32, u32, c.POINTER(_Rope),
+                                vp]),
+        "axh_kv_page_bytes": (u64, [u32, u32, u32]),
+        "axh_kv_append": (st, [vp, u32, vp, u64, vp, u64, c.POINTER(_KvCache),
+                               c.POINTER(_KvBatch), c.POINTER(_Rope), vp]),
+        "axh_kv_read": (st, [vp, c.POINTER(_KvCache), c.POINTER(_KvBatch), u32, vp, u64, vp, u64,
+                             vp]),
+        "axh_kv_attention_bytes": (u64, [c.POINTER(_KvCache), c.POINTER(_KvBatch),
+                                         c.POINTER(_AttentionOptions), u32]),
+        "axh_kv_attention": (st, [vp, u32, vp, u64, vp, u64, c.POINTER(_KvCache),
+                                  c.POINTER(_KvBatch), c.POINTER(_AttentionOptions), vp, u64, vp]),
         "axh_bench_loop": (st, [vp, c.POINTER(_BenchOp), u32, u32, u32, c.POINTER(c.c_float)]),
     }
     for name, (res, args) in sigs.items():
@@ -482,6 +524,126 @@ def expert_plan_bytes(n_tokens: int, top_k: int, n_experts: int) -> int:
     return int(load_library().axh_expert_plan_bytes(n_tokens, top_k, n_experts))
 
 
+@dataclass(frozen=True)
+class RopeOptions:
+    """A rotation by positions (axh_rope_options): the first `dim` elements of a head in pairs
+    (2i, 2i + 1), layout "pairs", or (i, i + dim / 2), "halves".  scale below 1 stretches the
+    positions; with extrapolate 1 fast frequencies are kept as they are (YaRN, with the
+    `original` context and beta_fast, beta_slow); magnitude multiplies the rotated elements."""
+
+    dim: int
+    layout: str = "pairs"
+    base: float = 10000.0
+    scale: float = 1.0
+    extrapolate: float = 0.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    original: int = 0
+    magnitude: float = 1.0
+
+    @functools.cached_property
+    def _c(self) -> _RopeOptions:
+        if self.layout not in ROPE_LAYOUTS:
+            raise ValueError(f"unknown rotation layout {self.layout!r}")
+        return _RopeOptions(self.dim, ROPE_LAYOUTS[self.layout], self.base, self.scale,
+                            self.extrapolate, self.beta_fast, self.beta_slow, self.original,
+                            self.magnitude)
+
+
+class RopeTable:
+    """A rotation's table on the device, made once; factors: dim / 2 divisors of the
+    frequencies (host values), as files of long-context models hold them."""
+
+    def __init__(self, ctx: "HipContext", options: RopeOptions,
+                 factors: Optional[Sequence[float]] = None):
+        o = options._c
+        n = int(load_library().axh_rope_table_bytes(options.dim))
+        if n == 0:
+            raise ValueError("dim must be even, 2 to 1024")
+        f = None
+        if factors is not None:
+            if len(factors) != options.dim // 2:
+                raise ValueError(f"{options.dim // 2} factors are wanted, not {len(factors)}")
+            f = (ctypes.c_float * len(factors))(*(float(x) for x in factors))
+        self.options, self.table = options, ctx.alloc(n)
+        try:
+            _check(ctx._lib.axh_rope_table(ctx._raw, ctypes.byref(o), f, self.table.ptr))
+        except DispatchError:
+            self.table.close()
+            raise
+        self._c = _Rope(self.table.ptr, options.dim, o.layout)
+
+    def close(self) -> None:
+        self.table.close()
+
+
+@dataclass(frozen=True)
+class KvCache:
+    """One layer's keys and values in pages (axh_kv_cache): k and v are the device memory of
+    n_pages pages of kv_page_bytes(...) each."""
+
+    k: object
+    v: object
+    n_pages: int
+    page_size: int
+    kv_heads: int
+    head_dim: int
+
+    @functools.cached_property
+    def _c(self) -> _KvCache:
+        return _KvCache(_ptr(self.k), _ptr(self.v), self.n_pages, self.page_size, self.kv_heads,
+                        self.head_dim)
+
+
+@dataclass(frozen=True)
+class KvBatch:
+    """New tokens of sequences (axh_kv_batch): int32 on the device, lengths[n_seqs] with the
+    new tokens, table[n_seqs][max_pages], and starts[n_seqs + 1] (None: a token each)."""
+
+    n_seqs: int
+    n_tokens: int
+    max_pages: int
+    lengths: object
+    table: object
+    starts: object = None
+
+    @functools.cached_property
+    def _c(self) -> _KvBatch:
+        return _KvBatch(self.n_seqs, self.n_tokens, self.max_pages, _ptr(self.starts),
+                        _ptr(self.lengths), _ptr(self.table))
+
+
+@dataclass(frozen=True)
+class AttentionOptions:
+    """axh_attention_options: query heads, the scores' scale, how many keys a row sees at most
+    (window, 0: all), and a bound of the lengths where one is known (max_length, 0: none)."""
+
+    n_heads: int
+    scale: float
+    window: int = 0
+    max_length: int = 0
+
+    @functools.cached_property
+    def _c(self) -> _AttentionOptions:
+        return _AttentionOptions(self.n_heads, self.scale, self.window, self.max_length)
+
+
+def kv_page_bytes(page_size: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of a page of keys (of values: the same)."""
+    n = int(load_library().axh_kv_page_bytes(page_size, kv_heads, head_dim))
+    if n == 0:
+        raise ValueError("pages have 16 to 4096 tokens (a power of two), a head_dim that is a "
+                         "multiple of 32 up to 256, and at least one head")
+    return n
+
+
+def kv_attention_bytes(cache: KvCache, batch: KvBatch, options: AttentionOptions,
+                       x_type: int = GGML_F32) -> int:
+    """Bytes of the workspace of a kv_attention call."""
+    return int(load_library().axh_kv_attention_bytes(
+        ctypes.byref(cache._c), ctypes.byref(batch._c), ctypes.byref(options._c), x_type))
+
+
 def mxfp4_matmul_kernel_name(n_rows: int, cols: int, batch: int, y_type: int = GGML_F32) -> str:
     """Entry point axh_mxfp4_matmul launches for this shape."""
     buf = ctypes.create_string_buffer(64)
@@ -577,6 +739,15 @@ def _ptr(obj) -> int:
     if hasattr(obj, "data_ptr"):
         return int(obj.data_ptr())
     raise TypeError(f"not a device pointer: {type(obj)!r}")
+
+
+def _nbytes(obj) -> int:
+    """Bytes of a DeviceBuffer or a tensor."""
+    if obj is None:
+        return 0
+    if hasattr(obj, "nbytes"):
+        return int(obj.nbytes)
+    raise TypeError(f"not a buffer of a known size: {type(obj)!r}")
 
 
 def _stream(s) -> Optional[int]:
@@ -1037,6 +1208,39 @@ class HipContext:
         _check(self._lib.axh_expert_combine(self._raw, y_type, _ptr(slots), _ptr(experts),
                                             _ptr(weights), _ptr(y), n_rows, n_tokens, top_k,
                                             n_experts, _stream(stream)))
+
+    # ---- rotary positions and the paged cache (include/axh_attn.h) ------------
+    def rope(self, x, y, positions, n_tokens: int, n_heads: int, head_dim: int, rope: RopeTable,
+             x_type: int = GGML_F32, x_stride: int = 0, y_stride: int = 0, stream=None) -> None:
+        """y = x (n_tokens x n_heads x head_dim) turned by positions (int32); y may be x."""
+        _check(self._lib.axh_rope_apply(self._raw, x_type, _ptr(x), x_stride, _ptr(y), y_stride,
+                                        _ptr(positions), n_tokens, n_heads, head_dim,
+                                        ctypes.byref(rope._c), _stream(stream)))
+
+    def kv_append(self, k, v, cache: KvCache, batch: KvBatch, rope: Optional[RopeTable] = None,
+                  x_type: int = GGML_F32, k_stride: int = 0, v_stride: int = 0,
+                  stream=None) -> None:
+        """The batch's rows k and v into the cache, in MXFP4; with rope, k turned first."""
+        _check(self._lib.axh_kv_append(self._raw, x_type, _ptr(k), k_stride, _ptr(v), v_stride,
+                                       ctypes.byref(cache._c), ctypes.byref(batch._c),
+                                       ctypes.byref(rope._c) if rope else None, _stream(stream)))
+
+    def kv_read(self, cache: KvCache, batch: KvBatch, k, v, y_type: int = GGML_F32,
+                k_stride: int = 0, v_stride: int = 0, stream=None) -> None:
+        """k and v = the batch's rows as the cache holds them."""
+        _check(self._lib.axh_kv_read(self._raw, ctypes.byref(cache._c), ctypes.byref(batch._c),
+                                     y_type, _ptr(k), k_stride, _ptr(v), v_stride,
+                                     _stream(stream)))
+
+    def kv_attention(self, q, y, cache: KvCache, batch: KvBatch, options: AttentionOptions,
+                     workspace, x_type: int = GGML_F32, q_stride: int = 0, y_stride: int = 0,
+                     stream=None) -> None:
+        """y = attention of q (n_tokens x n_heads x head_dim) over the cached tokens of their
+        sequences; workspace: a DeviceBuffer or tensor of kv_attention_bytes(...), or None."""
+        _check(self._lib.axh_kv_attention(
+            self._raw, x_type, _ptr(q), q_stride, _ptr(y), y_stride, ctypes.byref(cache._c),
+            ctypes.byref(batch._c), ctypes.byref(options._c), _ptr(workspace),
+            _nbytes(workspace), _stream(stream)))
 
     def cu_count(self) -> int:
         return int(self._lib.axh_cu_count(self._raw))

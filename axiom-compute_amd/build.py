@@ -44,7 +44,8 @@ HIP_FLAGS = [
 # kernarg load before its first memory request.
 KERNEL_FLAGS = ["-mllvm", "-amdgpu-kernarg-preload-count=16"]
 
-KERNELS = ["q4_matvec", "q4_matvec_wide", "q4_matmul", "mx_elem", "mx_matvec", "mx_matmul"]
+KERNELS = ["q4_matvec", "q4_matvec_wide", "q4_matmul", "mx_elem", "mx_matvec", "mx_matmul",
+           "kv_cache", "kv_attention"]
 
 # Host-only sanitizer build (g++ lines only).
 SAN_FLAGS = ["-fsanitize=address,undefined", "-fno-omit-frame-pointer",
@@ -93,7 +94,7 @@ def build_runtime(cos: dict[str, Path], sanitize: bool = False) -> Path:
         "-D__HIP_PLATFORM_AMD__", "-I", str(ROCM / "include"), "-I", str(ROOT / "include"),
         "-I", str(rt),
         str(rt / "axh_runtime.cpp"), str(rt / "axh_ops.cpp"), str(rt / "axh_mx.cpp"),
-        str(rt / "axh_gguf.cpp"),
+        str(rt / "axh_attn.cpp"), str(rt / "axh_gguf.cpp"),
         str(PKG / "csrc" / "tune" / "axh_tune.cpp"), str(PKG / "csrc" / "tune" / "axh_winners.cpp"),
         str(PKG / "csrc" / "check" / "axh_check.cpp"),
         str(embed_o), str(noalloc_o),

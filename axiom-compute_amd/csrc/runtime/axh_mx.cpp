@@ -5,6 +5,7 @@
 #include <cstdio>
 #include <cstring>
 #include <string>
+#include <utility>
 
 #include "axh_internal.h"
 #include "axh_mx.h"
@@ -12,14 +13,19 @@
 extern "C" const unsigned char axh_mx_elem_co_begin[], axh_mx_elem_co_end[];
 extern "C" const unsigned char axh_mx_matvec_co_begin[], axh_mx_matvec_co_end[];
 extern "C" const unsigned char axh_mx_matmul_co_begin[], axh_mx_matmul_co_end[];
+extern "C" const unsigned char axh_kv_cache_co_begin[], axh_kv_cache_co_end[];
+extern "C" const unsigned char axh_kv_attention_co_begin[], axh_kv_attention_co_end[];
 
 namespace axh {
 
 bool mx_code_object(uint32_t i, const void **co, size_t *bytes) {
-  const unsigned char *objs[3][2] = {{axh_mx_elem_co_begin, axh_mx_elem_co_end},
-                                     {axh_mx_matvec_co_begin, axh_mx_matvec_co_end},
-                                     {axh_mx_matmul_co_begin, axh_mx_matmul_co_end}};
-  if (i >= 3) return false;
+  const unsigned char *objs[kMxObjects][2] = {
+      {axh_mx_elem_co_begin, axh_mx_elem_co_end},
+      {axh_mx_matvec_co_begin, axh_mx_matvec_co_end},
+      {axh_mx_matmul_co_begin, axh_mx_matmul_co_end},
+      {axh_kv_cache_co_begin, axh_kv_cache_co_end},
+      {axh_kv_attention_co_begin, axh_kv_attention_co_end}};
+  if (i >= kMxObjects) return false;
   *co = objs[i][0];
   *bytes = (size_t)(objs[i][1] - objs[i][0]);
   return true;
@@ -27,7 +33,7 @@ bool mx_code_object(uint32_t i, const void **co, size_t *bytes) {
 
 namespace {
 
-enum Object { kElem = 0, kMatvec = 1, kMatmul = 2 };
+constexpr MxObject kElem = kMxElem, kMatvec = kMxMatvec, kMatmul = kMxMatmul;
 
 constexpr uint32_t kMaxCols = 1u << 22;    // the tiles' row offsets stay below 1 GiB
 constexpr uint64_t kMaxBuffer = 1ull << 31; // bytes of a buffer of the products' kernels
@@ -52,20 +58,8 @@ axh_status check_cols(uint32_t cols) {
   return AXH_OK;
 }
 
-axh_status launch(axh_context *ctx, Object obj, const std::string &name, uint64_t gx, uint64_t gy,
-                  uint32_t threads, uint32_t lds, void *const *bufs, uint32_t n_bufs,
-                  const uint32_t *words, uint32_t n_words, void *stream) {
-  // (a dimension's work-items are counted in 32 bits)
-  if (gx > ctx->core->max_wg[0] || gy > ctx->core->max_wg[1] || gx * threads > UINT32_MAX)
-    return fail(AXH_ERR_WORKGROUP_COUNT_EXCEEDS_LIMIT, name + ": grid exceeds the device limit");
-  hipSetDevice(ctx->core->device);
-  axh_kernel *k = nullptr;
-  axh_status s = mx_kernel(ctx, obj, name.c_str(), n_bufs, n_words * 4u, threads, &k);
-  if (s != AXH_OK) return s;
-  const uint32_t grid[3] = {(uint32_t)gx, (uint32_t)gy, 1};
-  s = launch_raw(k, grid, bufs, n_bufs, words, n_words * 4u, lds, pick_stream(ctx, stream));
-  return s == AXH_OK ? ok() : s;
-}
+// (the launches of this file)
+template <class... A> axh_status launch(A &&...args) { return mx_launch(std::forward<A>(args)...); }
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1u) / b); }
 
@@ -213,6 +207,21 @@ axh_status expert_launch(axh_context *ctx, const char *op, const char *type, boo
 }
 
 } // namespace
+
+axh_status mx_launch(axh_context *ctx, MxObject obj, const std::string &name, uint64_t gx, uint64_t gy,
+                  uint32_t threads, uint32_t lds, void *const *bufs, uint32_t n_bufs,
+                  const uint32_t *words, uint32_t n_words, void *stream) {
+  // (a dimension's work-items are counted in 32 bits)
+  if (gx > ctx->core->max_wg[0] || gy > ctx->core->max_wg[1] || gx * threads > UINT32_MAX)
+    return fail(AXH_ERR_WORKGROUP_COUNT_EXCEEDS_LIMIT, name + ": grid exceeds the device limit");
+  hipSetDevice(ctx->core->device);
+  axh_kernel *k = nullptr;
+  axh_status s = mx_kernel(ctx, obj, name.c_str(), n_bufs, n_words * 4u, threads, &k);
+  if (s != AXH_OK) return s;
+  const uint32_t grid[3] = {(uint32_t)gx, (uint32_t)gy, 1};
+  s = launch_raw(k, grid, bufs, n_bufs, words, n_words * 4u, lds, pick_stream(ctx, stream));
+  return s == AXH_OK ? ok() : s;
+}
 
 // Kernel `entry` of one of the code objects above, prepared once per context.
 axh_status mx_kernel(axh_context *ctx, uint32_t object, const char *entry, uint32_t n_buffers,
