@@ -3,6 +3,7 @@
 // kv_attention.hip.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -105,13 +106,17 @@ struct AttentionPlan {
 };
 
 AttentionPlan plan_attention(const axh_kv_cache *c, const axh_kv_batch *b,
-                             const axh_attention_options *o) {
+                             const axh_attention_options *o, uint32_t type) {
   AttentionPlan p{};
   const uint32_t per = o->n_heads / c->kv_heads;
-  p.kind = "r1";
-  p.rows = 16u;
-  const uint32_t step = 128u; // keys of a workgroup's step
-  const uint64_t target = 1024u;
+  const uint64_t mean = b->starts ? div_up((uint64_t)b->n_tokens * per, std::max(1u, b->n_seqs)) : per;
+  bool many = mean > 64u;
+  if (getenv("KVK")) many = getenv("KVK")[0] == 'm';
+  p.kind = many ? "many" : "few";
+  p.rows = many ? 128u : 16u;
+  const uint32_t step = many ? 32u : 128u; // keys of a workgroup's step
+  uint64_t target = many ? 512u : 1024u;
+  if (getenv("KVT")) target = atoi(getenv("KVT"));
   // Groups of a sequence's rows, its last one not full.
   p.groups = b->starts ? ((uint64_t)b->n_tokens * per + (uint64_t)b->n_seqs * (p.rows - 1u)) / p.rows
                        : (uint64_t)b->n_seqs * div_up(per, p.rows);
@@ -308,7 +313,7 @@ axh_status axh_kv_read(axh_context *ctx, const axh_kv_cache *cache, const axh_kv
 uint64_t axh_kv_attention_bytes(const axh_kv_cache *cache, const axh_kv_batch *batch,
                                 const axh_attention_options *options, uint32_t x_type) {
   if (check_attention(cache, batch, options, x_type) != AXH_OK) return 0;
-  return workspace_bytes_of(cache, batch, options, plan_attention(cache, batch, options));
+  return workspace_bytes_of(cache, batch, options, plan_attention(cache, batch, options, x_type));
 }
 
 axh_status axh_kv_attention(axh_context *ctx, uint32_t x_type, const void *q, uint64_t q_stride,
@@ -324,7 +329,7 @@ axh_status axh_kv_attention(axh_context *ctx, uint32_t x_type, const void *q, ui
   if (s == AXH_OK) s = check_rows("y", y, &y_stride, row, batch->n_tokens, type_size(x_type));
   if (s == AXH_OK) s = check_pointers(cache, batch);
   if (s != AXH_OK) return s;
-  const AttentionPlan p = plan_attention(cache, batch, options);
+  const AttentionPlan p = plan_attention(cache, batch, options, x_type);
   const uint64_t need = workspace_bytes_of(cache, batch, options, p);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return bad("the workspace must be 16-byte aligned and axh_kv_attention_bytes() long");
@@ -335,13 +340,15 @@ axh_status axh_kv_attention(axh_context *ctx, uint32_t x_type, const void *q, ui
   const uint32_t words[] = {batch->n_seqs, batch->n_tokens, batch->max_pages, cache->n_pages,
                             log2_of(cache->page_size), cache->kv_heads, cache->head_dim,
                             options->n_heads / cache->kv_heads, (uint32_t)q_stride,
-                            (uint32_t)y_stride, c_bits, options->window, p.chunk, p.splits};
+                            (uint32_t)y_stride, c_bits, options->window, p.chunk, p.splits,
+                            (uint32_t)axh_kv_page_bytes(cache->page_size, cache->kv_heads,
+                                                        cache->head_dim)};
   void *bufs[] = {mut(q), cache->k, cache->v, mut(batch->starts), mut(batch->lengths),
                   mut(batch->table), y, workspace};
   s = mx_launch(ctx, kKvAttention,
-                std::string("axh_kv_attention_") + p.kind + (cache->head_dim > 128u ? "_c2_" : "_c1_") +
-                    type,
-                p.groups * p.splits * cache->kv_heads, 1, 256, 0, bufs, 8, words, 14, stream);
+                std::string("axh_kv_attention_") + p.kind + "_d" +
+                    std::to_string(div_up(cache->head_dim, 64u) * 64u) + "_" + type,
+                p.groups * p.splits * cache->kv_heads, 1, 256, 0, bufs, 8, words, 15, stream);
   if (s != AXH_OK || p.splits <= 1u) return s;
   const uint32_t join[] = {batch->n_tokens, batch->n_seqs, options->n_heads, cache->head_dim,
                            (uint32_t)y_stride, p.splits};

@@ -20,8 +20,10 @@ from test_gpu_mx import BF16, F16, F32, ROUND, SIZE, Dev, _say, as_type, read_ou
 
 pytestmark = pytest.mark.gpu
 NAMES = {F32: "f32", F16: "f16", BF16: "bf16"}
-# rounding of the softmax's weights: one, two or three terms of bf16
-WEIGHTS = {BF16: 2.0 ** -8, F16: 2.0 ** -16, F32: 2.0 ** -24}
+# Rounding of the softmax's weights: once to bf16 or f16, three terms of bf16 for f32.  The sums
+# are those of the rounded weights w (1 + e): y is off by sum w e (v - y) to first order, at
+# most e (sum w |v| + |y|), and as |y| <= sum w |v|, by 2 e sum w |v|.
+WEIGHTS = {BF16: 2 * 2.0 ** -8, F16: 2 * 2.0 ** -11, F32: 2 * 2.0 ** -24}
 
 
 @pytest.fixture
