@@ -3,10 +3,8 @@
 // kv_attention.hip.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <cstring>
 #include <string>
-#include <vector>
 
 #include "axh_attn.h"
 #include "axh_internal.h"
@@ -17,6 +15,9 @@ namespace {
 
 constexpr uint32_t kMaxHeadDim = 256, kMaxRopeDim = 1024;
 constexpr uint64_t kMaxStride = 1ull << 31; // elements between tokens
+constexpr uint64_t kMaxPage = 1ull << 31;   // bytes of a page of keys
+constexpr float kLog2E = 1.44269504088896340736f;
+constexpr uint32_t kMaxSplits = 256;        // 64 of a wave of the kernel that joins them
 
 axh_status bad(const char *msg) { return fail(AXH_ERR_INVALID_ARGUMENT, msg); }
 bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1u)) == 0; }
@@ -56,7 +57,8 @@ axh_status check_rope(const axh_rope *r, uint32_t head_dim) {
 bool cache_sizes(uint32_t page_size, uint32_t kv_heads, uint32_t head_dim) {
   return page_size >= 16u && page_size <= 4096u && (page_size & (page_size - 1u)) == 0 &&
          kv_heads >= 1u && kv_heads <= 65536u && head_dim >= 32u && head_dim <= kMaxHeadDim &&
-         head_dim % 32u == 0;
+         head_dim % 32u == 0 &&
+         (uint64_t)page_size * kv_heads * (head_dim / 32u) * 17u < kMaxPage;
 }
 
 // Sizes only: what a workspace depends on.
@@ -64,7 +66,7 @@ axh_status check_sizes(const axh_kv_cache *c, const axh_kv_batch *b) {
   if (!c || !b) return bad("cache or batch is NULL");
   if (!cache_sizes(c->page_size, c->kv_heads, c->head_dim))
     return bad("a cache has pages of 16 to 4096 tokens (a power of two), 1 to 65536 heads, and a "
-               "head_dim that is a multiple of 32 up to 256");
+               "head_dim that is a multiple of 32 up to 256; a page is below 2^31 bytes");
   if (c->n_pages == 0 || c->n_pages >= 1u << 31) return bad("n_pages must be 1 to 2^31 - 1");
   if (b->max_pages == 0 || (uint64_t)b->max_pages * c->page_size >= 1ull << 31)
     return bad("max_pages must be at least 1, and max_pages * page_size below 2^31");
@@ -98,33 +100,64 @@ uint32_t heads_of_lane(uint64_t units, uint32_t n_heads) {
 }
 
 // ---- attention: the kernel and the split of the keys ----------------------------
+// Keep in sync with kv_attention.hip.
 struct AttentionPlan {
   const char *kind;
-  uint32_t rows;           // query rows of a workgroup
-  uint64_t groups;         // of them, at most
+  uint32_t rows;   // query rows of a workgroup
+  uint64_t groups; // of them, at most
   uint32_t chunk, splits;
 };
 
 AttentionPlan plan_attention(const axh_kv_cache *c, const axh_kv_batch *b,
                              const axh_attention_options *o, uint32_t type) {
   AttentionPlan p{};
-  const uint32_t per = o->n_heads / c->kv_heads;
-  const uint64_t mean = b->starts ? div_up((uint64_t)b->n_tokens * per, std::max(1u, b->n_seqs)) : per;
-  bool many = mean > 64u;
-  if (getenv("KVK")) many = getenv("KVK")[0] == 'm';
-  p.kind = many ? "many" : "few";
-  p.rows = many ? 128u : 16u;
-  const uint32_t step = many ? 32u : 128u; // keys of a workgroup's step
-  uint64_t target = many ? 512u : 1024u;
-  if (getenv("KVT")) target = atoi(getenv("KVT"));
-  // Groups of a sequence's rows, its last one not full.
-  p.groups = b->starts ? ((uint64_t)b->n_tokens * per + (uint64_t)b->n_seqs * (p.rows - 1u)) / p.rows
-                       : (uint64_t)b->n_seqs * div_up(per, p.rows);
+  const uint32_t per = o->n_heads / c->kv_heads, dims = (uint32_t)div_up(c->head_dim, 64u);
+  const bool f32 = type == AXH_GGML_F32;
+  const uint64_t rows = (uint64_t)b->n_tokens * per, seqs = std::max(1u, b->n_seqs);
+  const uint64_t mean = div_up(rows, seqs); // of a sequence
+  auto most = [&](uint32_t n) { // groups of n rows where each sequence's last one is not full
+    return b->starts ? (rows + seqs * (n - 1u)) / n : seqs * div_up(per, n);
+  };
+  auto expected = [&](uint32_t n) { // workgroups where sequences are equally long
+    return std::max<uint64_t>(1u, std::min(most(n), seqs * div_up(mean, n)) * c->kv_heads);
+  };
+  // 128 rows (which convert a key or a value once for 128 rows, not for 16 or 32, but go through
+  // all keys one after the other) where they are full and make 1024 workgroups; 32 rows (heads up
+  // to 128 in 16 bits: others have no registers for them) where they make 256.  Times (us) with
+  // 32 query and 8 key heads of 128 in bf16, queries to keys, 16 / 32 / 128 rows: 4096 to 4096
+  // 210 / 180 / 157; 3000 to 3000 (752 workgroups of 128 rows, three a CU at once, the longest as
+  // long as without the others) 127 / 116 / 165; 1024 to 6000 134 / 109 / 146; 256 to 6000 47 /
+  // 42 / 143; 128 to 6000 34 / 43 / 142.  4096 to 4096 in f32 440 / - / 470, heads of 256 in bf16
+  // 452 / - / 438, in f32 1197 / - / 768.
+  if (mean >= 128u && expected(128u) >= 1024u) {
+    p.kind = "many";
+    p.rows = 128u;
+  } else if (!f32 && dims <= 2u && mean > 16u && expected(32u) >= 256u) {
+    p.kind = "more";
+    p.rows = 32u;
+  } else {
+    p.kind = "few";
+    p.rows = 16u;
+  }
+  p.groups = most(p.rows);
   const uint64_t capacity = (uint64_t)b->max_pages * c->page_size;
   uint64_t keys = o->max_length ? std::min<uint64_t>(o->max_length, capacity) : capacity;
   if (o->window) keys = std::min<uint64_t>(keys, (uint64_t)o->window + 32u + div_up(p.rows, per));
-  const uint64_t want = std::max<uint64_t>(1u, target / std::max<uint64_t>(1u, p.groups * c->kv_heads));
-  p.chunk = (uint32_t)(div_up(div_up(keys, std::min<uint64_t>(want, 512u)), step) * step);
+  // A split's parts are written and read once more, and joined by another launch: nothing is
+  // split below 1024 keys (333 keys 6.9 us, in two 10.0; 1000 keys 9.3, in two 10.4), and beyond
+  // that into as many as make a workgroup a CU, two where that leaves them over 1024 keys each
+  // and three over 2048, as far as registers let a CU have them.  32 sequences of 8192 keys (256
+  // workgroups unsplit): 66 us, in two 48, three 44, four 46, eight 47.  One of 131072, 16 heads,
+  // f32: in 16 61, in 32 44, in 48 43, in 96 45.  One of 6000, 8 heads, 4 rows: in 8 11.1, in 32
+  // 9.7, in 48 10.6; 64 rows: in 4 15.2, in 8 12.6, in 12 14.6.
+  uint64_t splits = 1u;
+  if (p.rows == 16u && keys >= 1024u) {
+    const uint64_t wgs = expected(p.rows), each = keys * wgs / 256u;
+    const uint64_t room = f32 ? (dims == 1u ? 3u : dims == 4u ? 1u : 2u) : dims <= 2u ? 3u : 2u;
+    const uint64_t a_cu = std::min<uint64_t>(room, each > 2048u ? 3u : each > 1024u ? 2u : 1u);
+    splits = std::max<uint64_t>(1u, std::min<uint64_t>(kMaxSplits, 256u * a_cu / wgs));
+  }
+  p.chunk = (uint32_t)(div_up(div_up(keys, splits), 128u) * 128u);
   p.splits = (uint32_t)div_up(keys, p.chunk);
   return p;
 }
@@ -137,7 +170,8 @@ axh_status check_attention(const axh_kv_cache *c, const axh_kv_batch *b,
   if (!type_name(type)) return bad("x_type must be f32, f16 or bf16");
   if (o->n_heads == 0 || o->n_heads % c->kv_heads || o->n_heads > 65536u)
     return bad("n_heads must be a multiple of kv_heads, at most 65536");
-  if (!(o->scale > 0.0f) || !std::isfinite(o->scale)) return bad("scale must be positive and finite");
+  if (!(o->scale > 0.0f) || !std::isfinite(o->scale * kLog2E))
+    return bad("scale must be positive, and finite in base 2");
   if ((uint64_t)b->n_tokens * o->n_heads >= 1ull << 31) return bad("too many rows for one call");
   return AXH_OK;
 }
@@ -182,7 +216,7 @@ axh_status axh_rope_table(axh_context *ctx, const axh_rope_options *o, const flo
     low = std::max(0.0L, std::floor(pair_of(o->beta_fast)));
     high = std::min((long double)o->dim - 1.0L, std::ceil(pair_of(o->beta_slow)));
   }
-  std::vector<uint8_t> host(axh_rope_table_bytes(o->dim), 0);
+  uint8_t host[kMaxRopeDim / 2u * 8u + 8u] = {};
   for (uint32_t i = 0; i < pairs; ++i) {
     long double f = std::pow((long double)o->base, -2.0L * i / o->dim);
     if (factors) {
@@ -200,10 +234,10 @@ axh_status axh_rope_table(axh_context *ctx, const axh_rope_options *o, const flo
     // the fraction of a turn in 64 bits (a whole turn is none)
     const long double bits = std::round((turns - std::floor(turns)) * 18446744073709551616.0L);
     const uint64_t u = bits >= 18446744073709551616.0L ? 0u : (uint64_t)bits;
-    std::memcpy(host.data() + 8u * i, &u, 8);
+    std::memcpy(host + 8u * i, &u, 8);
   }
-  std::memcpy(host.data() + 8u * pairs, &o->magnitude, 4);
-  return axh_upload(ctx, table, host.data(), host.size());
+  std::memcpy(host + 8u * pairs, &o->magnitude, 4);
+  return axh_upload(ctx, table, host, axh_rope_table_bytes(o->dim));
 }
 
 axh_status axh_rope_apply(axh_context *ctx, uint32_t x_type, const void *x, uint64_t x_stride,
@@ -334,13 +368,15 @@ axh_status axh_kv_attention(axh_context *ctx, uint32_t x_type, const void *q, ui
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return bad("the workspace must be 16-byte aligned and axh_kv_attention_bytes() long");
   const std::string type = type_name(x_type);
-  const float c = options->scale * 1.44269504088896340736f; // log2 e
+  const float c = options->scale * kLog2E;
   uint32_t c_bits;
   std::memcpy(&c_bits, &c, 4);
+  // (positions are below 2^31)
+  const uint32_t window = options->window >= 1u << 31 ? 0u : options->window;
   const uint32_t words[] = {batch->n_seqs, batch->n_tokens, batch->max_pages, cache->n_pages,
                             log2_of(cache->page_size), cache->kv_heads, cache->head_dim,
                             options->n_heads / cache->kv_heads, (uint32_t)q_stride,
-                            (uint32_t)y_stride, c_bits, options->window, p.chunk, p.splits,
+                            (uint32_t)y_stride, c_bits, window, p.chunk, p.splits,
                             (uint32_t)axh_kv_page_bytes(cache->page_size, cache->kv_heads,
                                                         cache->head_dim)};
   void *bufs[] = {mut(q), cache->k, cache->v, mut(batch->starts), mut(batch->lengths),
@@ -353,9 +389,14 @@ axh_status axh_kv_attention(axh_context *ctx, uint32_t x_type, const void *q, ui
   const uint32_t join[] = {batch->n_tokens, batch->n_seqs, options->n_heads, cache->head_dim,
                            (uint32_t)y_stride, p.splits};
   void *joined[] = {workspace, mut(batch->starts), y};
-  return mx_launch(ctx, kKvAttention, "axh_kv_combine_" + type,
-                   (uint64_t)batch->n_tokens * options->n_heads, 1, 256, 0, joined, 3, join, 6,
-                   stream);
+  // Four waves a row where its parts are more than a wave reads at once.
+  const uint64_t all = (uint64_t)batch->n_tokens * options->n_heads;
+  const uint32_t per = p.splits > 8u ? 4u : 1u;
+  const uint32_t across = cache->head_dim > 128u ? 256u : cache->head_dim > 64u ? 128u : 64u;
+  return mx_launch(ctx, kKvAttention,
+                   "axh_kv_combine_w" + std::to_string(per) + "_d" + std::to_string(across) + "_" +
+                       type,
+                   div_up(all * per, 4u), 1, 256, 0, joined, 3, join, 6, stream);
 }
 
 } // extern "C"

@@ -68,7 +68,8 @@ axh_status axh_rope_apply(axh_context *ctx, uint32_t x_type, const void *x, uint
  * One layer's keys and values in MXFP4 (blocks of 32 along a head), in pages of
  * page_size tokens (a power of two, 16 to 4096), n_pages of them for the keys at k
  * and for the values at v (16-byte aligned), axh_kv_page_bytes() each.  head_dim is
- * a multiple of 32, 32 to 256.  A page has, for each head in turn,
+ * a multiple of 32, 32 to 256, and a page of the keys is below 2^31 bytes.  It has, for
+ * each head in turn,
  *   keys:    page_size rows of head_dim / 2 bytes of codes, then page_size rows
  *            of head_dim / 32 scale bytes;
  *   values:  for each four tokens, 4 bytes of codes (8 elements) of each of them,
@@ -87,7 +88,8 @@ axh_status axh_rope_apply(axh_context *ctx, uint32_t x_type, const void *x, uint
  * be written to them is left out, and so is what would be read; the same goes for
  * positions below 0 (more tokens than the length) and from max_pages * page_size
  * (below 2^31) on.  Tokens before starts[0] or from starts[n_seqs] on belong to no
- * sequence, and no call touches their rows.  starts must not decrease. */
+ * sequence, and no call touches their rows.  starts must not decrease, from 0 on and up
+ * to n_tokens.  A length below 0 is one of 0. */
 typedef struct axh_kv_cache {
     void *k;
     void *v;
@@ -126,10 +128,14 @@ axh_status axh_kv_read(axh_context *ctx, const axh_kv_cache *cache, const axh_kv
  * head_dim of one type, strides between tokens; y apart from q.  A row that sees no key, or none
  * whose score is above -inf, is 0.  Keys that a row does not see have no part in
  * it, whatever their bytes; NaN blocks of those that it sees make it NaN.
- *   Scores, sums and the output are f32.  The matrix instructions multiply bf16: a
- * cached value and a bf16 q are exact in it, an f16 or f32 q is two or three terms
- * that add up to it exactly; the softmax's weights are rounded to one, two or three
- * terms for bf16, f16 and f32 (within 2^-8, 2^-16, 2^-24 relative).
+ *   Scores, maxima and sums are f32 and the output is rounded once.  The matrix instructions
+ * multiply bf16 for bf16 and f32 operands, f16 for f16: a cached value is exact in bf16, a
+ * q in its own type, an f32 q as three bf16 terms that add up to it.  The softmax's weights
+ * are rounded once to bf16 (2^-8) or f16 (2^-11), or are three bf16 terms (2^-24), and the
+ * sums are of the rounded weights.  For f16 operands cached values count as f16: those
+ * below 2^-14 are rounded to multiples of 2^-24, and a block with values of 2^16 and more
+ * (scale bytes above 140) makes the rows that see it infinite or NaN; weights below 2^-32
+ * of a row's largest may count as 0.
  *   max_length bounds the lengths as far as the caller knows (0: max_pages *
  * page_size).  With it the keys are split among workgroups; sequences beyond it are
  * computed all the same.  workspace: axh_kv_attention_bytes() for the same cache
@@ -137,8 +143,8 @@ axh_status axh_kv_read(axh_context *ctx, const axh_kv_cache *cache, const axh_kv
  * done: calls that may overlap need one each, and so do graphs that do. */
 typedef struct axh_attention_options {
     uint32_t n_heads;    /* a multiple of kv_heads */
-    float scale;         /* above 0 */
-    uint32_t window;     /* 0: none */
+    float scale;         /* above 0, below 2.3e38 */
+    uint32_t window;     /* 0: none, and so is 2^31 and more */
     uint32_t max_length;
 } axh_attention_options;
 uint64_t axh_kv_attention_bytes(const axh_kv_cache *cache, const axh_kv_batch *batch,

@@ -154,9 +154,10 @@ class Batch:
                              None if plain else d[2])
 
 
-def device_cache(dev, axc, cache):
-    return axc.KvCache(dev.up(cache.k), dev.up(cache.v), cache.n_pages, cache.page_size,
-                       cache.heads, cache.dim)
+def device_cache(dev, axc, cache, copies=1):
+    k, v = (np.tile(x, (1, copies, 1)) for x in (cache.k, cache.v))
+    return axc.KvCache(dev.up(k), dev.up(v), cache.n_pages, cache.page_size, cache.heads * copies,
+                       cache.dim)
 
 
 def fill(cache, batch, seed, loud=()):
@@ -255,14 +256,18 @@ def test_append_and_read(ctx, dev, axc, t, new, lengths, page, heads, dim, rotat
 
 # ---- attention ---------------------------------------------------------------------------
 def run_attention(ctx, dev, axc, t, cache, dc, b, heads, window=0, max_length=0, seed=11, q=None,
-                  q_stride=0, y_stride=0, scale=None):
-    """(output, exact, tolerance) of a call; rows of no sequence are checked to be left."""
+                  q_stride=0, y_stride=0, scale=None, copies=1):
+    """(output, exact, tolerance) of a call; rows of no sequence are checked to be left.  copies:
+    `dc` has the cache's heads so often, one copy after the other, and so has the call; all
+    copies are checked to be equal."""
     dim = cache.dim
     scale = float(np.float32(scale or dim ** -0.5))
     x = rows_of(seed, b.n_tokens, heads, dim) if q is None else q
-    dq, x = strided(dev, x, t, q_stride)
-    o = axc.AttentionOptions(n_heads=heads, scale=scale, window=window, max_length=max_length)
-    row = heads * dim
+    dq, _ = strided(dev, np.tile(x, (1, copies, 1)), t, q_stride)
+    x = as_type(x, t)[1]
+    o = axc.AttentionOptions(n_heads=heads * copies, scale=scale, window=window,
+                             max_length=max_length)
+    row = heads * copies * dim
     size = b.n_tokens * (y_stride or row) * SIZE[t]
     dy = dev.out(size)
     n = axc.kv_attention_bytes(dc, b.c, o, t)
@@ -282,7 +287,9 @@ def run_attention(ctx, dev, axc, t, cache, dc, b, heads, window=0, max_length=0,
     free = [i for i, a in enumerate(at) if a is None]
     assert np.array_equal(y[free], blank[free])
     mine = [i for i, a in enumerate(at) if a is not None]
-    y = y[:, :row].reshape(x.shape)[mine]
+    y = y[:, :row].reshape(b.n_tokens, copies, heads, dim)[mine]
+    assert np.array_equal(y, np.repeat(y[:, :1], copies, 1), equal_nan=True)
+    y = y[:, 0]
     exact, terms = exact[mine], terms[:, mine]
     tol = KV.attention_bound(terms, dim, WEIGHTS[t])
     return y, exact, tol + ROUND[t] * (np.abs(exact) + tol) + (2.0 ** -24 if t == F16 else 0)
@@ -560,3 +567,157 @@ def test_calls_on_the_default_stream(ctx, dev, axc):
     ctx.kv_attention(dev.up(x), dy, dc, b.c, o, ws, stream=axc.DEFAULT_STREAM)
     ctx.synchronize(axc.DEFAULT_STREAM)
     assert np.array_equal(dev.down(dy, x.nbytes, np.float32, x.shape), y)
+
+
+# ---- prompts: heads enough that workgroups have 32 and 128 rows ----------------------------
+def copies_for(b, per, kv, rows):
+    """Copies of the heads that make as many workgroups of `rows` rows as such calls have, by
+    their mean length: 256 of 32, 1024 of 128."""
+    seqs = len(b.new)
+    mean = -(-b.n_tokens * per // seqs)
+    assert mean >= {32: 17, 128: 128}[rows]
+    groups = min(seqs * -(-mean // rows), (b.n_tokens * per + seqs * (rows - 1)) // rows)
+    return -(-{32: 256, 128: 1024}[rows] // (groups * kv))
+
+
+def attend_copies(ctx, dev, axc, t, cache, b, heads, rows, **kw):
+    n = copies_for(b, heads // cache.heads, cache.heads, rows)
+    return run_attention(ctx, dev, axc, t, cache, device_cache(dev, axc, cache, n), b, heads,
+                         copies=n, **kw)
+
+
+# new tokens, lengths, page, kv heads, query heads, dim, window
+PROMPTS = [
+    ([130, 300], [131, 500], 64, 1, 1, 128, 0),
+    ([40], [333], 32, 1, 5, 64, 0),
+    ([64, 1, 70], [200, 300, 70], 32, 1, 5, 224, 33),
+    ([300], [300], 16, 1, 1, 32, 64),
+    ([100, 0, 200], [60, 9, 700], 16, 1, 3, 96, 100),  # forty tokens before a sequence's first
+    ([129], [129], 256, 2, 4, 256, 0),
+    ([250], [1100], 128, 1, 1, 192, 0),
+    ([150, 140], [150, 2], 16, 1, 1, 160, 1),
+]
+
+
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+@pytest.mark.parametrize("new,lengths,page,kv,heads,dim,window", PROMPTS)
+@pytest.mark.parametrize("rows", [32, 128])
+def test_attention_of_prompts(ctx, dev, axc, rows, t, new, lengths, page, kv, heads, dim, window):
+    _say(f"{rows} rows, {NAMES[t]} {new} of {lengths}, {heads}/{kv}x{dim}, window {window}")
+    b = Batch(dev, axc, 70, new, lengths, page, before=1, after=2)
+    cache = KV.Cache(b.n_pages, page, kv, dim)
+    fill(cache, b, 71)
+    check(*attend_copies(ctx, dev, axc, t, cache, b, heads, rows, window=window))
+
+
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+@pytest.mark.parametrize("dim", [64, 96, 256])
+@pytest.mark.parametrize("rows", [32, 128])
+def test_nan_blocks_in_prompts(ctx, dev, axc, rows, t, dim):
+    """NaN blocks where some rows of a workgroup see them and others do not."""
+    _say(f"NaN blocks, {rows} rows, {NAMES[t]} {dim}")
+    b = Batch(dev, axc, 72, [90, 70], [190, 75], 16)
+    last = dim // 32 - 1
+    loud = [(0, 150, 0, last, "v"), (0, 3, 1, 0, "v"), (0, 188, 1, 0, "k"), (1, 64, 0, last, "v"),
+            (1, 5, 1, 0, "k"), (1, 40, 1, last, "v")]
+    cache = KV.Cache(b.n_pages, 16, 2, dim)
+    fill(cache, b, 73, loud)
+    for window in (0, 30):
+        y, exact, tol = attend_copies(ctx, dev, axc, t, cache, b, 4, rows, window=window)
+        assert np.isnan(exact).any() and not np.isnan(exact).all()
+        check(y, exact, tol)
+
+
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+@pytest.mark.parametrize("rows", [32, 128])
+def test_pages_and_rows_that_are_not_there_in_prompts(ctx, dev, axc, rows, t):
+    """Missing pages, a sequence without any, lengths beyond the table, rows of it that see
+    nothing, and what a page that is not there has in the cache: NaN."""
+    _say(f"missing pages, {rows} rows, {NAMES[t]}")
+    b = Batch(dev, axc, 74, [140, 160, 130], [500, 190, 150], 16, max_pages=20,
+              missing=[(0, 1, -1), (0, 2, None), (0, 5, 1 << 30), (0, 6, -(1 << 31)),
+                       (2, 0, -1), (2, 8, -1)])
+    b.table[1] = -1
+    b.d_table = dev.up(b.table)
+    b.c = axc.KvBatch(3, b.n_tokens, b.max_pages, b.d_lengths, b.d_table, b.c.starts)
+    cache = KV.Cache(b.n_pages, 16, 1, 64)
+    fill(cache, b, 75)  # (pages that no row of the table names are NaN all over)
+    y, exact, tol = attend_copies(ctx, dev, axc, t, cache, b, 1, rows)
+    check(y, exact, tol)
+    assert (y[140:300] == 0).all() and not np.isnan(exact).any()
+
+
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+@pytest.mark.parametrize("rows", [32, 128])
+def test_scores_of_any_size_in_prompts(ctx, dev, axc, rows, t):
+    """Maxima that rise along the keys by more than the slack, fall, or stay, differently in
+    neighbouring rows; queries that are infinite or NaN beside them."""
+    _say(f"scores of any size, {rows} rows, {NAMES[t]}")
+    n = 300
+    b = Batch(dev, axc, 76, [n], [n], 32)
+    cache = KV.Cache(b.n_pages, 32, 1, 64)
+    v = rows_of(77, n, 1, 64)
+    for p in range(n):
+        k = np.zeros((1, 64))
+        k[0, 0], k[0, 1] = 1.0 * (p // 50), 1.0 * (6 - p // 50)
+        cache.write(b.table, 0, p, k, v[p])
+    q = np.zeros((n, 1, 64), np.float32)
+    q[0::4, 0, 0], q[1::4, 0, 1], q[2::4, 0, 0], q[3::4, 0, 2] = 400.0, 400.0, -30.0, 1.0
+    # Weights e^-400 and less are below what the kernels can hold.  In f32 and bf16 one that
+    # falls below 2^-126 may become 0; the sum of weights is at least 1, that of the largest or
+    # more, so a key's part of y is off by 2^-126 |v|, and the sum's by as much times |y| <= max
+    # |v|.  In f16 a weight is off by at most half of the smallest number, 2^-25, the largest at
+    # least 2^7: 2^-32 in the place of 2^-126.
+    lost = 2 * n * np.abs(MX.decode(*MX.quantize(v.reshape(-1, 64)))).max()
+    lost *= 2.0 ** -32 if t == F16 else 2.0 ** -126
+    y, exact, tol = attend_copies(ctx, dev, axc, t, cache, b, 1, rows, q=q, scale=1.0)
+    check(y, exact, tol + lost)
+    q[17, 0, 5], q[133, 0, 7], q[260, 0, 9] = np.nan, np.inf, -np.inf
+    y, exact, tol = attend_copies(ctx, dev, axc, t, cache, b, 1, rows, q=q, scale=1.0)
+    loud = [17, 133, 260]
+    assert np.isnan(y[loud]).all()
+    quiet = np.setdiff1d(np.arange(n), loud)
+    check(y[quiet], exact[quiet], tol[quiet] + lost)
+
+
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+@pytest.mark.parametrize("rows", [32, 128])
+def test_strides_of_prompts(ctx, dev, axc, rows, t):
+    _say(f"strides, {rows} rows, {NAMES[t]}")
+    b = Batch(dev, axc, 78, [131], [140], 16)
+    cache = KV.Cache(b.n_pages, 16, 1, 32)
+    fill(cache, b, 79)
+    row = 2 * 32 * copies_for(b, 2, 1, rows)
+    check(*attend_copies(ctx, dev, axc, t, cache, b, 2, rows, q_stride=row + 200,
+                         y_stride=row + 8))
+
+
+@pytest.mark.parametrize("new", [[1], [20], [130]])
+def test_windows_and_lengths_up_to_2_to_the_31(ctx, dev, axc, new):
+    """Windows of 2^31 and more hide nothing; a window of 2^31 - 1 neither."""
+    _say(f"large windows, {new}")
+    b = Batch(dev, axc, 80, new, [200], 16)
+    cache = KV.Cache(b.n_pages, 16, 2, 64)
+    fill(cache, b, 81)
+    for rows in ([128] if new[0] > 128 else []) + [16]:
+        n = copies_for(b, 1, 2, 128) if rows == 128 else 1
+        dc = device_cache(dev, axc, cache, n)
+        plain = run_attention(ctx, dev, axc, F32, cache, dc, b, 2, copies=n)
+        check(*plain)
+        for window in ((1 << 31) - 1, 1 << 31, (1 << 32) - 1):
+            y = run_attention(ctx, dev, axc, F32, cache, dc, b, 2, window, copies=n)[0]
+            assert np.array_equal(y, plain[0])
+
+
+@pytest.mark.parametrize("length", [-1, -5, -(1 << 31)])
+@pytest.mark.parametrize("t", [BF16, F32])
+def test_lengths_below_zero(ctx, dev, axc, t, length):
+    """Such a sequence has no cached token: its rows are 0, and none is written or read."""
+    _say(f"a length of {length}")
+    b = Batch(dev, axc, 82, [3, 2], [length, 40], 16)
+    cache = KV.Cache(b.n_pages, 16, 1, 64)
+    fill(cache, b, 83)
+    b.lengths = np.maximum(b.lengths, 0)  # (as the formula has it)
+    y, exact, tol = run_attention(ctx, dev, axc, t, cache, device_cache(dev, axc, cache), b, 2)
+    check(y, exact, tol)
+    assert (y[:3] == 0).all()

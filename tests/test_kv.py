@@ -195,3 +195,16 @@ def test_rotations_that_are_refused(calls, axc):
         assert table(**bad) == INVALID, bad
     with pytest.raises(ValueError):
         axc.RopeOptions(4, layout="thirds")._c
+
+
+def test_sizes_past_what_the_kernels_count(calls, axc):
+    """Pages of 2^31 bytes and more (the kernels count a page's bytes in 32 bits), scales whose
+    base-2 form is infinite."""
+    lib = calls.lib
+    assert lib.axh_kv_page_bytes(4096, 3855, 256) == 4096 * 3855 * 8 * 17  # below 2^31
+    assert lib.axh_kv_page_bytes(4096, 3856, 256) == 0
+    assert lib.axh_kv_page_bytes(4096, 65536, 256) == 0
+    big = dict(page_size=4096, kv_heads=3856, head_dim=256)
+    assert calls.attend(cache=big, options=dict(n_heads=3856)) == INVALID
+    assert calls.append(cache=big) == INVALID
+    assert calls.attend(options=dict(scale=3.0e38)) == INVALID
