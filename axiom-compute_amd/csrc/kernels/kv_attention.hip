@@ -1240,9 +1240,9 @@ template <class T, int kDim> struct Many {
 // ---------------------------------------------------------------------------
 // The splits' parts of a row, added: kWaves waves a row, each at most 64 parts, whose maxima
 // and sums are a lane's each; kAcross lanes (of 4 elements) a part, the others beside them, all
-// parts of 8 rounds in flight together: what it takes is the latency of two reads behind a launch.
-// 16 rows of 47 parts, 128 elements 2.0 us less than with one wave that reads the maxima first;
-// up to 8 parts of a row, one wave is as fast, and four rows a workgroup are fewer workgroups.
+// parts of 8 rounds in flight together with the maxima.  16 rows of 47 parts, 128 elements 2.0 us
+// less than with one wave that reads the maxima first; up to 8 parts of a row, one wave is as fast, and four
+// rows a workgroup are fewer workgroups.
 // ---------------------------------------------------------------------------
 template <class T, int kWaves, int kAcross>
 __device__ __forceinline__ void combine_body(const float *ws, const int32_t *starts, uint8_t *y,
@@ -1251,8 +1251,8 @@ __device__ __forceinline__ void combine_body(const float *ws, const int32_t *sta
                                              float *lds) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, part = wave % kWaves;
   const uint64_t n = (uint64_t)n_tokens * n_heads;
-  const uint64_t id = (uint64_t)blockIdx.x * (4u / kWaves) + wave / kWaves;
-  const uint32_t token = (uint32_t)(id / n_heads), h = (uint32_t)(id - (uint64_t)token * n_heads);
+  const uint32_t id = blockIdx.x * (4u / kWaves) + wave / kWaves; // (below 2^31)
+  const uint32_t token = id / n_heads, h = id - token * n_heads;
   bool real = id < n;
   if (real && starts) real = (int32_t)token >= starts[0] && (int32_t)token < starts[n_seqs];
   // the wave's parts
@@ -1264,7 +1264,21 @@ __device__ __forceinline__ void combine_body(const float *ws, const int32_t *sta
     top = ms[0];
     total = ms[1];
   }
-  const uint64_t has = __ballot(total != 0.0f); // (or NaN)
+  const uint32_t at = lane % kAcross, beside = lane / kAcross, e = 4u * at;
+  constexpr uint32_t kBeside = 64u / kAcross, kRound = 8u * kBeside;
+  const float *parts = ws + parts_at(n, splits);
+  f32x4_t v[8];
+  auto ask = [&](uint32_t s) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t k = s + kBeside * i + beside;
+      v[i] = (f32x4_t){0, 0, 0, 0};
+      if (real && k < mine && e < dim)
+        v[i] = *reinterpret_cast<const f32x4_t *>(parts + ((uint64_t)(s0 + k) * n + id) * dim + e);
+    }
+  };
+  ask(0u);
+  const uint64_t has = __ballot(total != 0.0f); // (or NaN; what empty parts hold is not used)
   float most = has >> lane & 1u ? top : kLowest;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
@@ -1272,25 +1286,16 @@ __device__ __forceinline__ void combine_body(const float *ws, const int32_t *sta
   total *= f;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-  const uint32_t at = lane % kAcross, beside = lane / kAcross, e = 4u * at;
-  constexpr uint32_t kBeside = 64u / kAcross;
-  const float *parts = ws + parts_at(n, splits);
   f32x4_t x = {0, 0, 0, 0};
-  for (uint32_t s = 0; s < mine; s += 8u * kBeside) {
-    f32x4_t v[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t k = s + kBeside * i + beside;
-      v[i] = (f32x4_t){0, 0, 0, 0};
-      if (k < mine && (has >> k & 1u) && e < dim)
-        v[i] = *reinterpret_cast<const f32x4_t *>(parts + ((uint64_t)(s0 + k) * n + id) * dim + e);
-    }
+  for (uint32_t s = 0; s < mine; s += kRound) {
+    if (s) ask(s);
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
       const uint32_t k = s + kBeside * i + beside;
       const float g = __shfl(f, (int)(k < 64u ? k : 63u));
+      const bool on = k < mine && (has >> k & 1u);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(v[i][j], k < mine ? g : 0.0f, x[j]);
+      for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(on ? v[i][j] : 0.0f, on ? g : 0.0f, x[j]);
     }
   }
 #pragma unroll

@@ -106,7 +106,9 @@ __device__ __forceinline__ void rope_body(const uint8_t *x, uint8_t *y, const in
 // block of 32: its largest magnitude is two DPP steps away, and the converting
 // instruction divides by the block's power of two, so an element is rounded once.
 // blockIdx.y 0: keys, turned first where there is a table (angles once a lane, for `per`
-// heads; the partners of the other half are read beside the lane's own), 1: values.
+// heads; the partners of the other half are read beside the lane's own), 1: values.  A head's
+// elements are asked for before the one before it is written, the first's and the angles' turns
+// before the token's place is known.
 // ---------------------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ void append_body(const uint8_t *k, const uint8_t *v, uint8_t *cache_k,
@@ -121,48 +123,71 @@ __device__ __forceinline__ void append_body(const uint8_t *k, const uint8_t *v, 
   const uint32_t id = blockIdx.x * 256u + threadIdx.x;
   const uint32_t unit = id % units, rest = id / units;
   const uint32_t token = rest / groups, h0 = rest % groups * per;
-  if (token >= n_tokens) return; // (whole quads: units is a multiple of 4)
-  const Place at = place_of(starts, lengths, n_seqs, token);
+  const bool real = token < n_tokens; // (whole quads: units is a multiple of 4)
+  const uint32_t h1 = h0 + per < g.kv_heads ? h0 + per : g.kv_heads;
+  const uint8_t *xr = (values ? v : k) + (uint64_t)token * (values ? v_stride : k_stride) * T::kBytes;
+  const uint32_t e0 = unit * 8u, half = dim / 2u;
+  // element e0 + i times c[i], and its partner times s[i]
+  const bool turn = !values && turns && e0 < dim;
+  const bool halves = layout != 0u, wide = dim % 16u == 0u; // (of halves: partners are 8 in a row)
+  const uint32_t partner = e0 < half ? e0 + half : e0 - half;
+  float x[8] = {}, o[8] = {};
+  auto ask = [&](uint32_t h, float *xs, float *os) {
+    const uint8_t *head = xr + (uint64_t)h * g.dim * T::kBytes;
+    load8<T>(head + e0 * T::kBytes, xs);
+    if (!turn || !halves) return;
+    if (wide) {
+      load8<T>(head + partner * T::kBytes, os);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t e = e0 + i;
+        if (e < dim) os[i] = load1<T>(head + (e < half ? e + half : e - half) * T::kBytes);
+      }
+    }
+  };
+  if (real) ask(h0, x, o);
+  // (of the pair, where both its elements are the lane's: once)
+  const Rope rope(turns, dim, layout);
+  uint64_t angle[8] = {};
+  if (turn) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t e = e0 + i;
+      if (e < dim && (halves || i % 2u == 0u))
+        angle[i] = rope.turns[!halves ? e >> 1 : e < half ? e : e - half];
+    }
+  }
+  const Place at = place_of(starts, lengths, n_seqs, n_tokens, token);
+  if (!real) return;
   const int32_t page = page_of(table, g, max_pages, at);
   if (page < 0) return;
   const uint32_t row = (uint32_t)at.pos & (g.page_rows() - 1u);
-  const uint32_t h1 = h0 + per < g.kv_heads ? h0 + per : g.kv_heads;
-  const uint8_t *xr = (values ? v : k) + (uint64_t)token * (values ? v_stride : k_stride) * T::kBytes;
-  const uint32_t e0 = unit * 8u;
-  // element e0 + i times c[i], and its partner times s[i]
-  const bool turn = !values && turns && e0 < dim;
   float c[8], s[8];
-  uint32_t partner[8];
-  bool wide = false;
-  if (turn) {
-    const Rope rope(turns, dim, layout);
+  if (turn) { // (elements behind the rotated ones are left alone below)
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t e = e0 + i, half = dim / 2u;
-      c[i] = 1.0f;
-      s[i] = 0.0f;
-      partner[i] = e;
-      if (e < dim) {
-        const bool second = rope.halves ? e >= half : (e & 1u);
-        rope.at(rope.halves ? (second ? e - half : e) : e >> 1, at.pos, c[i], s[i]);
-        partner[i] = rope.halves ? (second ? e - half : e + half) : e ^ 1u;
-        if (!second) s[i] = -s[i];
+      if (halves) {
+        rope.of(angle[i], at.pos, c[i], s[i]);
+        if (e0 + i < half) s[i] = -s[i];
+      } else if (i % 2u == 0u) {
+        rope.of(angle[i], at.pos, c[i], s[i]);
+        c[i + 1] = c[i];
+        s[i + 1] = s[i];
+        s[i] = -s[i];
       }
     }
-    wide = rope.halves && dim % 16u == 0u;
   }
   uint8_t *out = (values ? cache_v : cache_k) + g.head_offset((uint32_t)page, 0);
+  const uint32_t code_at = values ? g.value_code(row, unit) : g.key_code(row, unit);
+  const uint32_t scale_at = values ? g.value_scale(row, unit >> 2) : g.key_scale(row, unit >> 2);
   for (uint32_t h = h0; h < h1; ++h) {
-    const uint8_t *head = xr + (uint64_t)h * g.dim * T::kBytes;
-    float x[8];
-    load8<T>(head + e0 * T::kBytes, x);
+    float next[8], other[8];
+    if (h + 1u < h1) ask(h + 1u, next, other);
     if (turn) {
-      float o[8];
-      if (wide) {
-        load8<T>(head + partner[0] * T::kBytes, o);
-      } else {
+      if (!halves) {
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) o[i] = load1<T>(head + partner[i] * T::kBytes);
+        for (uint32_t i = 0; i < 8; ++i) o[i] = x[i ^ 1u];
       }
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i)
@@ -174,22 +199,25 @@ __device__ __forceinline__ void append_body(const uint8_t *k, const uint8_t *v, 
       const uint32_t b = __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu;
       m = b > m ? b : m;
     }
-    uint32_t o = dpp_u32<kXor1>(m);
-    m = o > m ? o : m;
-    o = dpp_u32<kXor2>(m);
-    m = o > m ? o : m;
+    uint32_t w = dpp_u32<kXor1>(m);
+    m = w > m ? w : m;
+    w = dpp_u32<kXor2>(m);
+    m = w > m ? w : m;
     const uint32_t e = mx_scale_byte(m);
     const uint32_t codes = e == 255u ? 0u : fp4_pack8(x, mx_divisor(e));
     uint8_t *base = out + (uint64_t)h * g.head_bytes();
-    *reinterpret_cast<uint32_t *>(base + (values ? g.value_code(row, unit)
-                                                 : g.key_code(row, unit))) = codes;
-    if ((unit & 3u) == 0u)
-      base[values ? g.value_scale(row, unit >> 2) : g.key_scale(row, unit >> 2)] = (uint8_t)e;
+    *reinterpret_cast<uint32_t *>(base + code_at) = codes;
+    if ((unit & 3u) == 0u) base[scale_at] = (uint8_t)e;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      x[i] = next[i];
+      o[i] = other[i];
+    }
   }
 }
 
-// Rows of the cache as f32, f16 or bf16: a lane has 8 elements of a token's heads, bound
-// by the stores.
+// Rows of the cache as f32, f16 or bf16: a lane has 8 elements of a token's heads, four heads'
+// codes and scales in flight; bound by the stores.
 template <class T>
 __device__ __forceinline__ void read_body(const uint8_t *cache_k, const uint8_t *cache_v,
                                           const int32_t *starts, const int32_t *lengths,
@@ -202,34 +230,34 @@ __device__ __forceinline__ void read_body(const uint8_t *cache_k, const uint8_t 
   const uint32_t id = blockIdx.x * 256u + threadIdx.x;
   const uint32_t unit = id % units, rest = id / units;
   const uint32_t token = rest / groups, h0 = rest % groups * per;
-  if (token >= n_tokens) return;
-  const Place at = place_of(starts, lengths, n_seqs, token);
-  if (at.seq < 0) return; // of no sequence
+  const Place at = place_of(starts, lengths, n_seqs, n_tokens, token);
+  if (token >= n_tokens || at.seq < 0) return; // (of no sequence)
   const int32_t page = page_of(table, g, max_pages, at);
   const uint32_t row = (uint32_t)at.pos & (g.page_rows() - 1u);
   const uint32_t h1 = h0 + per < g.kv_heads ? h0 + per : g.kv_heads;
   uint8_t *yr = (values ? v : k) + (uint64_t)token * (values ? v_stride : k_stride) * T::kBytes;
   const uint8_t *in = (values ? cache_v : cache_k) + g.head_offset(page < 0 ? 0u : (uint32_t)page, 0);
-  for (uint32_t h = h0; h < h1; ++h) {
-    float x[8] = {};
-    if (page >= 0) {
-      const uint8_t *base = in + (uint64_t)h * g.head_bytes();
-      const uint32_t codes = *reinterpret_cast<const uint32_t *>(
-          base + (values ? g.value_code(row, unit) : g.key_code(row, unit)));
-      const float s = e8m0_to_f32(base[values ? g.value_scale(row, unit >> 2)
-                                              : g.key_scale(row, unit >> 2)]);
-      const f32x2_t p0 = fp4_pair<0>(codes), p1 = fp4_pair<1>(codes), p2 = fp4_pair<2>(codes),
-                    p3 = fp4_pair<3>(codes);
-      x[0] = p0.x * s;
-      x[1] = p0.y * s;
-      x[2] = p1.x * s;
-      x[3] = p1.y * s;
-      x[4] = p2.x * s;
-      x[5] = p2.y * s;
-      x[6] = p3.x * s;
-      x[7] = p3.y * s;
+  const uint32_t code_at = values ? g.value_code(row, unit) : g.key_code(row, unit);
+  const uint32_t scale_at = values ? g.value_scale(row, unit >> 2) : g.key_scale(row, unit >> 2);
+  for (uint32_t h = h0; h < h1; h += 4u) {
+    uint32_t codes[4], scales[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint8_t *base = in + (uint64_t)(h + i) * g.head_bytes();
+      const bool on = page >= 0 && h + i < h1;
+      codes[i] = on ? *reinterpret_cast<const uint32_t *>(base + code_at) : 0u;
+      scales[i] = on ? base[scale_at] : 0u;
     }
-    store8<T>(yr + ((uint64_t)h * g.dim + unit * 8u) * T::kBytes, x);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      if (h + i >= h1) break;
+      const float s = e8m0_to_f32(scales[i]);
+      const f32x2_t p0 = fp4_pair<0>(codes[i]), p1 = fp4_pair<1>(codes[i]),
+                    p2 = fp4_pair<2>(codes[i]), p3 = fp4_pair<3>(codes[i]);
+      const float x[8] = {p0.x * s, p0.y * s, p1.x * s, p1.y * s,
+                          p2.x * s, p2.y * s, p3.x * s, p3.y * s};
+      store8<T>(yr + ((uint64_t)(h + i) * g.dim + unit * 8u) * T::kBytes, x);
+    }
   }
 }
 

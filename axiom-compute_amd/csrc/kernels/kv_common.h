@@ -41,19 +41,40 @@ struct Place {
   int32_t seq, pos;
 };
 // starts NULL: one token a sequence.  starts[] does not decrease, so the last s with
-// starts[s] <= token is the one that holds it (those before it may be empty).
+// starts[s] <= token is the one that holds it (those before it may be empty).  All lanes of
+// the wave call it, also those whose token is none of the batch.  Up to 64 sequences, a lane
+// reads one's start and length, and the search is among lanes: two reads in place of a chain of
+// log2 n_seqs + 2.
 __device__ __forceinline__ Place place_of(const int32_t *starts, const int32_t *lengths,
-                                          uint32_t n_seqs, uint32_t token) {
-  if (!starts) return {(int32_t)token, lengths[token] - 1};
-  uint32_t lo = 0, hi = n_seqs; // starts[lo] <= token < starts[hi], if it is in a sequence
-  while (hi - lo > 1u) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (starts[mid] <= (int32_t)token) lo = mid;
-    else hi = mid;
+                                          uint32_t n_seqs, uint32_t n_tokens, uint32_t token) {
+  if (!starts) return {(int32_t)token, token < n_tokens ? lengths[token] - 1 : -1};
+  uint32_t lo = 0;
+  int32_t first, last, len;
+  if (n_seqs <= 64u) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const int32_t start = lane < n_seqs ? starts[lane] : 0, end = starts[n_seqs];
+    const int32_t mine = lane < n_seqs ? lengths[lane] : 0;
+#pragma unroll
+    for (uint32_t step = 32; step; step >>= 1) {
+      const int32_t v = __shfl(start, (int)((lo + step) & 63u));
+      if (lo + step < n_seqs && v <= (int32_t)token) lo += step;
+    }
+    first = __shfl(start, (int)lo);
+    last = __shfl(start, (int)((lo + 1u) & 63u));
+    if (lo + 1u == n_seqs) last = end;
+    len = __shfl(mine, (int)lo);
+  } else {
+    uint32_t hi = n_seqs; // starts[lo] <= token < starts[hi], if it is in a sequence
+    while (hi - lo > 1u) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if (starts[mid] <= (int32_t)token) lo = mid;
+      else hi = mid;
+    }
+    first = starts[lo];
+    last = starts[lo + 1u];
+    len = lengths[lo];
   }
-  const int32_t first = starts[lo], last = starts[lo + 1u];
   if ((int32_t)token < first || (int32_t)token >= last) return {-1, -1};
-  const int32_t len = lengths[lo];
   const int32_t pos = (int32_t)((uint32_t)len - (uint32_t)last + token);
   return {(int32_t)lo, pos < len ? pos : -1};
 }
@@ -139,7 +160,10 @@ struct Rope {
       : turns(static_cast<const uint64_t *>(table)), dim(d), halves(layout != 0u),
         magnitude(table ? *reinterpret_cast<const float *>(turns + d / 2u) : 1.0f) {}
   __device__ __forceinline__ void at(uint32_t pair, int32_t pos, float &c, float &s) const {
-    rotation(turns[pair], pos, c, s);
+    of(turns[pair], pos, c, s);
+  }
+  __device__ __forceinline__ void of(uint64_t turn, int32_t pos, float &c, float &s) const {
+    rotation(turn, pos, c, s);
     c *= magnitude;
     s *= magnitude;
   }

@@ -92,10 +92,12 @@ uint32_t log2_of(uint32_t n) {
   return s;
 }
 
-// Heads that a lane goes through with its angles and its token's place: as many as leave
-// 2^18 lanes.
-uint32_t heads_of_lane(uint64_t units, uint32_t n_heads) {
-  const uint64_t per = std::max<uint64_t>(1u, std::min<uint64_t>(n_heads, units >> 18));
+// Heads that a lane goes through with its token's place and angles: as many as leave 2^least
+// lanes.  Rotations 2^18 (4096 x 40 x 128 in bf16 14.4 us, with 2^16 20.5), rows in and out of the
+// cache 2^16 (9001 x 4 x 96 in f16, turned, in and out again 13.9 us, with 2^18 19.2: an angle
+// takes the time of a head's elements).
+uint32_t heads_of_lane(uint64_t units, uint32_t n_heads, uint32_t least) {
+  const uint64_t per = std::max<uint64_t>(1u, std::min<uint64_t>(n_heads, units >> least));
   return (uint32_t)div_up(n_heads, div_up(n_heads, per));
 }
 
@@ -271,7 +273,7 @@ axh_status axh_rope_apply(axh_context *ctx, uint32_t x_type, const void *x, uint
                               : rope->dim / (wide ? 8u : 2u);
   const uint32_t rest = x == y ? 0u : (head_dim - rope->dim) / (wide ? 8u : 1u);
   const uint32_t units = turned + rest;
-  const uint32_t per = heads_of_lane((uint64_t)n_tokens * units * n_heads, n_heads);
+  const uint32_t per = heads_of_lane((uint64_t)n_tokens * units * n_heads, n_heads, 18u);
   const uint64_t groups = div_up(n_heads, per);
   const uint32_t words[] = {n_tokens, n_heads,   head_dim, (uint32_t)x_stride, (uint32_t)y_stride,
                             rope->dim, rope->layout, units, per, (uint32_t)groups};
@@ -303,7 +305,7 @@ axh_status axh_kv_append(axh_context *ctx, uint32_t x_type, const void *k, uint6
   if (s != AXH_OK) return s;
   const uint32_t units = cache->head_dim / 8u;
   const uint32_t per =
-      heads_of_lane((uint64_t)batch->n_tokens * units * cache->kv_heads, cache->kv_heads);
+      heads_of_lane((uint64_t)batch->n_tokens * units * cache->kv_heads, cache->kv_heads, 16u);
   const uint64_t groups = div_up(cache->kv_heads, per);
   const uint32_t words[] = {batch->n_tokens, batch->n_seqs, batch->max_pages, cache->n_pages,
                             log2_of(cache->page_size), cache->kv_heads, cache->head_dim,
@@ -332,7 +334,7 @@ axh_status axh_kv_read(axh_context *ctx, const axh_kv_cache *cache, const axh_kv
   if (s != AXH_OK) return s;
   const uint32_t units = cache->head_dim / 8u;
   const uint32_t per =
-      heads_of_lane((uint64_t)batch->n_tokens * units * cache->kv_heads, cache->kv_heads);
+      heads_of_lane((uint64_t)batch->n_tokens * units * cache->kv_heads, cache->kv_heads, 16u);
   const uint64_t groups = div_up(cache->kv_heads, per);
   const uint32_t words[] = {batch->n_tokens, batch->n_seqs, batch->max_pages, cache->n_pages,
                             log2_of(cache->page_size), cache->kv_heads, cache->head_dim,
