@@ -65,7 +65,7 @@ __device__ __forceinline__ u32x4_t flags(uint32_t bits) {
   return w;
 }
 
-constexpr float kLowest = -3e38f; // below every score, and finite: no -inf less -inf
+constexpr float kLowest = -0x1.fffffep127f; // no finite score is below it, and no -inf less -inf
 constexpr float kSlack = 8.0f;    // how far (log2) a score may pass its row's maximum
 
 // What the products are made of for each type of q: terms of an operand, the two codes of a

@@ -128,7 +128,9 @@ axh_status axh_kv_read(axh_context *ctx, const axh_kv_cache *cache, const axh_kv
  * head_dim of one type, strides between tokens; y apart from q.  A row that sees no key, or none
  * whose score is above -inf, is 0.  Keys that a row does not see have no part in
  * it, whatever their bytes; NaN blocks of those that it sees make it NaN.
- *   Scores, maxima and sums are f32 and the output is rounded once.  The matrix instructions
+ *   Scores, maxima and sums are f32 and the output is rounded once.  Scores (scaled) are meant to
+ * be below 2^23 ln 2 = 5.8e6 in magnitude, where f32 still tells halves apart in base 2: a
+ * row with larger ones may be 0 or NaN.  The matrix instructions
  * multiply bf16 for bf16 and f32 operands, f16 for f16: a cached value is exact in bf16, a
  * q in its own type, an f32 q as three bf16 terms that add up to it.  The softmax's weights
  * are rounded once to bf16 (2^-8) or f16 (2^-11), or are three bf16 terms (2^-24), and the

@@ -721,3 +721,56 @@ def test_lengths_below_zero(ctx, dev, axc, t, length):
     y, exact, tol = run_attention(ctx, dev, axc, t, cache, device_cache(dev, axc, cache), b, 2)
     check(y, exact, tol)
     assert (y[:3] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [16, 32, 128])
+@pytest.mark.parametrize("factor", [-5.8e6, -1.0, 5.8e6])
+def test_scores_up_to_their_limit(ctx, dev, axc, rows, factor):
+    """All keys equal, so that every row is the mean of the values that it sees, whatever the
+    score, up to 2^23 in base 2 (5.8e6 log2 e = 8.37e6).  The weights are all the same, 1 but for
+    the rounding of the maximum (2^-24 of it, half a unit: a factor that the sum has too), so only
+    the weights' terms round, by 2^-24 each, and the sums, by 2^-22 a term, and the division."""
+    _say(f"scores of {factor}, {rows} rows")
+    n = 150 if rows > 16 else 40
+    b = Batch(dev, axc, 84, [n], [n], 16)
+    cache = KV.Cache(b.n_pages, 16, 1, 32)
+    v = rows_of(85, n, 1, 32)
+    k = np.zeros((1, 32))
+    k[0, 0] = 1.0
+    for p in range(n):
+        cache.write(b.table, 0, p, k, v[p])
+    q = np.zeros((n, 1, 32), np.float32)
+    q[:, 0, 0] = factor
+    c = copies_for(b, 1, 1, rows) if rows > 16 else 1
+    y = run_attention(ctx, dev, axc, F32, cache, device_cache(dev, axc, cache, c), b, 1, q=q,
+                      scale=1.0, copies=c)[0]
+    values = MX.decode(*MX.quantize(v[:, 0])).astype(np.float64)
+    many = np.arange(1, n + 1)[:, None]
+    exact = np.cumsum(values, 0) / many
+    # (the sum of up to n terms is n times a mean of them: n 2^-22 of the mean magnitude)
+    tol = (2.0 ** -22 * many + 2.0 ** -22) * np.cumsum(np.abs(values), 0) / many
+    assert (np.abs(y[:, 0] - exact) <= tol).all(), np.max(np.abs(y[:, 0] - exact) - tol)
+
+
+@pytest.mark.parametrize("rows", [16, 32, 128])
+def test_blocks_that_f16_does_not_hold(ctx, dev, axc, rows):
+    """f16 operands: values of 2^16 and more make the rows that see them infinite or NaN, in
+    their block, and no other row or element; values below f16's normal range are off by at
+    most half of its smallest step."""
+    _say(f"values outside of f16, {rows} rows")
+    n = 150 if rows > 16 else 40
+    b = Batch(dev, axc, 86, [n], [n], 16)
+    cache = KV.Cache(b.n_pages, 16, 1, 64)
+    fill(cache, b, 87)
+    for p, block, byte in ((21, 1, 141), (7, 0, 100), (12, 1, 103)):
+        codes, scale = cache._bytes(p % 16, True)
+        cache.v[b.table[0, p // 16], 0, scale[block]] = byte
+        if byte == 141:
+            cache.v[b.table[0, p // 16], 0, codes[16 * block:16 * block + 16]] = 0x77
+    c = copies_for(b, 1, 1, rows) if rows > 16 else 1
+    y, exact, tol = run_attention(ctx, dev, axc, F16, cache, device_cache(dev, axc, cache, c), b, 1,
+                                  copies=c)
+    loud = np.zeros(y.shape, bool)
+    loud[21:, :, 32:] = True
+    assert not np.isfinite(y[loud]).any()
+    check(y[~loud], exact[~loud], tol[~loud] + 2.0 ** -25)
