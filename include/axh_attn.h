@@ -59,7 +59,8 @@ axh_status axh_rope_table(axh_context *ctx, const axh_rope_options *options, con
                           void *table);
 /* y = x, n_tokens x n_heads x head_dim of one type, turned by positions[token] (int32,
  * also negative); strides between tokens; elements from dim on are copied.  In place (y
- * == x, equal strides) or apart.  In f32, rounded once.  head_dim at most 1024. */
+ * == x, equal strides) or apart.  In f32, rounded once.  head_dim at most 1024.  The gradient
+ * of x is that of y turned by the negated positions, with the same table. */
 axh_status axh_rope_apply(axh_context *ctx, uint32_t x_type, const void *x, uint64_t x_stride,
                           void *y, uint64_t y_stride, const int32_t *positions, uint32_t n_tokens,
                           uint32_t n_heads, uint32_t head_dim, const axh_rope *rope, void *stream);

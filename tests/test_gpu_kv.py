@@ -126,6 +126,41 @@ def test_rope_of_far_positions_is_that_of_near_ones(ctx, dev, axc):
     table.close()
 
 
+@pytest.mark.parametrize("layout", ["pairs", "halves"])
+def test_the_gradient_of_a_rotation(ctx, dev, axc, layout):
+    """dL/dx = the rotation of dL/dy by the negated positions: against the formula's transpose,
+    and against differences of L = sum g y along a direction (L is linear in x: they are exact
+    but for rounding)."""
+    _say(f"a rotation's gradient, {layout}")
+    tokens, heads, head_dim, dim = 9, 3, 40, 32
+    pos = np.array([0, 1, 2, 1000, -7, 65535, 1 << 20, (1 << 31) - 1, 12345], np.int32)
+    table = axc.RopeTable(ctx, axc.RopeOptions(dim=dim, layout=layout, scale=0.25, magnitude=1.125))
+    x, g, way = (rows_of(s, tokens, heads, head_dim) for s in (50, 51, 52))
+
+    def turned(v, positions):
+        out = dev.out(v.nbytes)
+        ctx.rope(dev.up(v), out, dev.up(positions), tokens, heads, head_dim, table)
+        ctx.synchronize()
+        return dev.down(out, v.nbytes, np.float32, v.shape).astype(np.float64)
+
+    dx = turned(g, -pos)
+    f = KV.frequencies(dim, scale=0.25)
+    # the formula's transpose, column by column: y = R x, so R^T g
+    eye = np.eye(head_dim)[None].repeat(tokens, 0)
+    r = KV.rotate(eye, pos, f, layout == "halves", 1.125)  # row j: R e_j
+    exact = np.einsum("tji,thi->thj", r, g.astype(np.float64))
+    size = np.einsum("tji,thi->thj", np.abs(r), np.abs(g).astype(np.float64))
+    assert (np.abs(dx - exact) <= 2.0 ** -21 * size + 2.0 ** -24 * np.abs(exact)).all()
+    step = 0.5
+    up, down = (turned((x + s * way).astype(np.float32), pos) for s in (step, -step))
+    change = ((up - down) * g).sum() / (2 * step)
+    # x +- way / 2 rounds by 2^-24 of each, a turned element by 2^-21 of its pair, all times g
+    most = (np.abs(x) + np.abs(way)).max() * 2 * 1.125
+    tol = np.abs(g).sum() * most * (2.0 ** -20) / step
+    assert abs(change - (dx * way).sum()) <= tol
+    table.close()
+
+
 # ---- the cache -------------------------------------------------------------------------
 class Batch:
     """A batch on the host and on the device: new tokens and lengths of sequences, pages in
@@ -774,3 +809,62 @@ def test_blocks_that_f16_does_not_hold(ctx, dev, axc, rows):
     loud[21:, :, 32:] = True
     assert not np.isfinite(y[loud]).any()
     check(y[~loud], exact[~loud], tol[~loud] + 2.0 ** -25)
+
+
+def test_calls_at_once(ctx, dev, axc):
+    """Two batches over one cache, on two streams at once and in two graphs replayed in turn, each
+    with its own workspace: what they give alone, bit for bit."""
+    _say("calls at once")
+    heads, kv, dim = 16, 4, 128
+    batches = [Batch(dev, axc, 90, [1, 1, 1], [2900, 1500, 60], 16),
+               Batch(dev, axc, 90, [7, 1, 30], [2900, 1500, 60], 16)]
+    cache = KV.Cache(batches[0].n_pages, 16, kv, dim)
+    rng = np.random.default_rng(91)
+    cache.k[:] = rng.integers(0, 256, cache.k.shape, dtype=np.uint8)
+    cache.v[:] = rng.integers(0, 256, cache.v.shape, dtype=np.uint8)
+    for pages, values in ((cache.k, False), (cache.v, True)):  # scales near 1
+        for p in range(16):
+            pages[:, :, cache._bytes(p, values)[1]] = 126
+    dc = device_cache(dev, axc, cache)
+    o = axc.AttentionOptions(n_heads=heads, scale=dim ** -0.5)
+    calls = []
+    for i, b in enumerate(batches):
+        x = rows_of(92 + i, b.n_tokens, heads, dim)
+        n = axc.kv_attention_bytes(dc, b.c, o)
+        assert n > 0  # (its keys are split)
+        calls.append((dev.up(x), dev.out(x.nbytes), b, ctx.alloc(n), x))
+
+    def run(i, stream=None):
+        q, y, b, ws, _ = calls[i]
+        ctx.kv_attention(q, y, dc, b.c, o, ws, stream=stream)
+
+    def result(i):
+        return dev.down(calls[i][1], calls[i][4].nbytes, np.float32, calls[i][4].shape)
+
+    alone = []
+    for i in range(2):
+        run(i)
+        ctx.synchronize()
+        alone.append(result(i))
+        assert np.isfinite(alone[i]).all() and np.abs(alone[i]).max() > 0
+    for _ in range(20):
+        run(0)
+        run(1, axc.DEFAULT_STREAM)
+    ctx.synchronize()
+    ctx.synchronize(axc.DEFAULT_STREAM)
+    assert np.array_equal(result(0), alone[0]) and np.array_equal(result(1), alone[1])
+    graphs = [ctx.capture(lambda i=i: run(i)) for i in range(2)]
+    for _ in range(5):
+        for i in range(2):
+            ctx.upload(calls[i][1], np.zeros_like(calls[i][4]))
+        ctx.synchronize()
+        for g in graphs:
+            g.launch()
+        ctx.synchronize()
+        assert np.array_equal(result(0), alone[0]) and np.array_equal(result(1), alone[1])
+        run(0)
+    ctx.synchronize()
+    for g in graphs:
+        g.close()
+    for c in calls:
+        c[3].close()
