@@ -321,7 +321,7 @@ template <class T, int kDim, int kRows> struct Rows {
   Group at;
   uint32_t rows, row0;           // of the sequence; the wave's first
   int32_t all_from, all_to;      // keys that all rows of the wave see
-  // Where a lane's codes and scales are from where a tile's are.
+  // Where a lane's codes and scales are in a page, of its first tile.
   uint32_t kc[kChunks], ks[kChunks], vc[kChunks], vs[kChunks];
   const uint8_t *kh, *vh;        // the head's part of page 0
   const int32_t *pages_of;       // the sequence's row of the table
@@ -359,9 +359,9 @@ template <class T, int kDim, int kRows> struct Rows {
       if (8u * kd >= dim) kd = 0;
       if (8u * vd >= dim) vd = 0;
       kc[c] = a.g.key_code(m, kd);
-      ks[c] = m * (dim / 32u) + (kd >> 2);
+      ks[c] = a.g.key_scale(m, kd >> 2);
       vc[c] = a.g.value_code(4u * grp, vd);
-      vs[c] = grp * (dim / 8u) + (vd >> 2) * 4u;
+      vs[c] = a.g.value_scale(4u * grp, vd >> 2);
     }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
@@ -420,14 +420,13 @@ template <class T, int kDim, int kRows> struct Rows {
     auto at = [&](uint32_t id) { return (uint64_t)(id < a.g.n_pages ? id : 0u) * a.page_bytes; };
     return {{at(p.id[0]), at(p.id[1])}, {p.id[0] < a.g.n_pages, p.id[1] < a.g.n_pages}};
   }
-  // A tile's page; codes and scales of the tile from `codes` and `scales` on, of keys as of
-  // values.
+  // A tile's page; codes and scales of the tile so much further on, of keys as of values.
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(const uint8_t *base, const Pages &p,
                                                          int T16, uint32_t t, uint32_t &codes,
                                                          uint32_t &scales) const {
     const uint32_t row = (t + 16u * T16) & (a.g.page_rows() - 1u);
     codes = a.g.key_code(row, 0u);
-    scales = a.g.key_scale(row, 0u);
+    scales = row * (a.g.dim / 32u);
     return rsrc(base + p.at[T16], a.g.head_bytes());
   }
   __device__ __forceinline__ void load_keys(Raw<kChunks> &r, const Pages &p, uint32_t t) const {
