@@ -633,7 +633,7 @@ def kv_page_bytes(page_size: int, kv_heads: int, head_dim: int) -> int:
     n = int(load_library().axh_kv_page_bytes(page_size, kv_heads, head_dim))
     if n == 0:
         raise ValueError("pages have 16 to 4096 tokens (a power of two), a head_dim that is a "
-                         "multiple of 32 up to 256, and at least one head")
+                         "multiple of 32 up to 256, at least one head, and less than 2^31 bytes")
     return n
 
 
